@@ -23,6 +23,7 @@ ADV_ELAUNCH = -5
 ADV_SPACE_AFFINE = 0
 ADV_SPACE_IDENTITY = 1
 ADV_SPACE_AFFINE_RCP = 2
+ADV_F32, ADV_BF16, ADV_F16 = 0, 1, 2
 ABI_VERSION = 11
 
 
@@ -56,6 +57,8 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
+_U = ctypes.c_uint64
 _SP = ctypes.POINTER(AdvSpace)
 _F3 = ctypes.POINTER(ctypes.c_float)
 _CI = ctypes.POINTER(AdvCleanIndex)
@@ -133,8 +136,16 @@ SIGNATURES = {
     "adv_conv2d_wino4_ksplit_f32": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "adv_conv3d_wino4_prep_weights_f32": [_P, _P, _I, _I, _I, _P],
     "adv_conv3d_wino4_f32": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "adv_dropout_fwd": [_P, _P, _P, _L, _L, _I, _D, _U, _P, _L, _I, _P],
+    "adv_dropout_bwd": [_P, _P, _P, _P, _P, _L, _L, _I, _D, _U, _P, _L, _P],
+    "adv_mx4_quantize": [_P, _P, _P, _L, _L, _I, _P],
+    "adv_mx4_dequantize": [_P, _P, _P, _L, _L, _I, _P],
+    "adv_mx4_linear": [_P, _P, _P, _P, _P, _P, _L, _L, _L, _I, _I, _P],
+    "adv_mx4_linear_dgrad": [_P, _P, _P, _P, _P, _L, _L, _L, _I, _P],
 }
 _OTHER = {
+    "adv_mx4_code_bytes": ([_L, _L], ctypes.c_int64),
+    "adv_dropout_bwd_workspace_floats": ([_L, _L, _I], ctypes.c_int64),
     "adv_abi_version": ([], _I),
     "adv_build_has_test_hooks": ([], _I),
     "adv_roi_align_bwd_workspace_ints": ([_I, _I, _I, _I, _I, _I, _I], ctypes.c_int64),

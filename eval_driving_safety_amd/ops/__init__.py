@@ -10,6 +10,8 @@
   volume   after the 3D convolutions: depth regression, 5-D grid sampling, bilinear up-sampling, bird's-eye-view fold, focal loss (csrc/volume.hip, csrc/resize.hip)
   boxes    the proposal / target stage of a Stereo R-CNN step: IoU rows, regression targets, decode + clip, size partition, roi sampling,
            the RPN head's list packing, the attack objective's six-term chain (csrc/boxes.hip)
+  dropout  a fully connected head's bias + dropout + ReLU, mask from a counter-based generator (csrc/dropout.hip)
+  mx4      MXFP4 matrices: quantisation, product, input gradient - a head with four-bit weights (csrc/mx4.hip)
   elementwise  ReLU backward, the ResNet stem's bias + ReLU + max-pooling (csrc/volume.hip)
 
 Each function is the counterpart of one inline block of the reference's attack scripts (cited per function) and keeps its argument
@@ -26,5 +28,7 @@ from .wino4 import *       # noqa: F401,F403
 from .align import *       # noqa: F401,F403
 from .volume import *       # noqa: F401,F403
 from .boxes import *       # noqa: F401,F403
+from .dropout import *       # noqa: F401,F403
+from .mx4 import *       # noqa: F401,F403
 
-SOURCES = tuple(__import__("os").path.join(__import__("os").path.dirname(__file__), n + ".py") for n in ("_base", "elementwise", "pixel", "psv", "roi", "conv3d", "conv2d", "wino4", "align", "volume", "boxes"))
+SOURCES = tuple(__import__("os").path.join(__import__("os").path.dirname(__file__), n + ".py") for n in ("_base", "elementwise", "pixel", "psv", "roi", "conv3d", "conv2d", "wino4", "align", "volume", "boxes", "dropout", "mx4"))

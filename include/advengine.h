@@ -627,6 +627,43 @@ ADV_API int adv_box_decode_stereo_f32(const float* anchors, const float* deltas,
 /* out[i] = y[i] > 0 ? grad[i] : 0  (the backward of a ReLU fused into a convolution's epilogue; out may alias grad). */
 ADV_API int adv_relu_backward_f32(const float* grad, const float* y, float* out, int64_t n, adv_stream_t stream);
 
+/* ---- fully connected heads (the scenario-context classifiers, dynamic_vehicles/Model.py:15-34 and driving_constraint/Model.py:15-30; a
+ *      detector's RoI head).  Tensors are contiguous, of the type `dtype`, and need that type's own alignment only; arithmetic is float32 with
+ *      one rounding to the type at the end.  Buffers that an entry point writes must not overlap its other buffers, except where said. */
+enum { ADV_F32 = 0, ADV_BF16 = 1, ADV_F16 = 2 };
+
+/* Dropout with the bias before it and the ReLU behind it, the mask from a counter-based generator and never stored:
+ *     word(i) = output i % 4 of Philox4x32 (seven rounds) of the counter (i / 4, step) under the key `seed`; element i (its place in memory)
+ *     is kept if word(i) >= round(p * 2^32);  y = relu?(kept ? (x + bias) / (1 - p) : 0).  p in [0, 1]; p = 1 keeps nothing.
+ *     A dropped element is 0 whatever x holds there.  x [rows, cols]; bias [cols] or NULL; y may be x itself.
+ *     step_at: a DEVICE int64 that holds the step, read when the kernel runs (a captured graph then draws a new mask whenever the caller
+ *     has moved it on), or NULL: the step is `step` (>= 0).
+ *     _bwd: gx [rows, cols] from gy - pass y, the forward's output, if and only if the forward had relu != 0 -, and gbias [cols] (NULL: not
+ *     wanted) = the sums of gx's columns before rounding, in a fixed order, with `workspace` of _workspace_floats floats (0: NULL allowed).
+ *     gx may be gy itself. */
+ADV_API int adv_dropout_fwd(const void* x, const void* bias, void* y, int64_t rows, int64_t cols, int dtype, double p, uint64_t seed,
+                            const int64_t* step_at, int64_t step, int relu, adv_stream_t stream);
+ADV_API int64_t adv_dropout_bwd_workspace_floats(int64_t rows, int64_t cols, int dtype);
+ADV_API int adv_dropout_bwd(const void* gy, const void* y, void* gx, void* gbias, float* workspace, int64_t rows, int64_t cols, int dtype, double p,
+                            uint64_t seed, const int64_t* step_at, int64_t step, adv_stream_t stream);
+
+/* Matrices held in MXFP4: 32 consecutive values of a row as 4-bit floats (e2m1) under one power of two (e8m0).
+ *     codes   [panels][rows][128] bytes, panels = ceil(cols / 256), the value of an even column in the low nibble; 16-byte aligned,
+ *             adv_mx4_code_bytes bytes.  scales [panels][rows][8] bytes (a sixteenth of that), 8-byte aligned.  Columns behind `cols` are zero.
+ *     rows <= 2^20, cols <= 2^22.
+ *   _quantize   per block e = clamp(floor(log2 max|x|) - 2, -127, 127), codes nearest-even(x / 2^e) saturated at 6, scale byte e + 127; a block that
+ *               holds a NaN or an infinity gets scale byte 255: it is NaN as a whole.
+ *   _linear     y [m, n] = relu?(X . W^T + bias) for X [m, k] and W [n, k] in MXFP4, bias [n] or NULL; products exact, sums float32.
+ *   _linear_dgrad  gx [m, k] = G . W, G [m, n] = gy, 0 where mask (NULL, or laid out like gy: the layer's ReLU output) is <= 0; gy enters exactly,
+ *               sums float32. */
+ADV_API int64_t adv_mx4_code_bytes(int64_t rows, int64_t cols);
+ADV_API int adv_mx4_quantize(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, int dtype, adv_stream_t stream);
+ADV_API int adv_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int64_t cols, int dtype, adv_stream_t stream);
+ADV_API int adv_mx4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias, void* y,
+                           int64_t m, int64_t n, int64_t k, int dtype, int relu, adv_stream_t stream);
+ADV_API int adv_mx4_linear_dgrad(const void* gy, const void* mask, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, int64_t m, int64_t n,
+                                 int64_t k, int dtype, adv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

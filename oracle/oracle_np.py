@@ -820,3 +820,80 @@ def box_decode_clip(src, d, width, height):
     out[:, 0::2] = np.clip(out[:, 0::2], 0, np.float32(width - 1))
     out[:, 1::2] = np.clip(out[:, 1::2], 0, np.float32(height - 1))
     return out
+
+
+# ------------------------------------------------------------------------------------------------ fully connected heads
+def philox4x32(i4, step, seed, rounds=7):
+    """the four output words (uint32 values in uint64 arrays [n,4]) of the counters (i4, step) under ``seed`` (Salmon et al., SC'11, section 3)"""
+    lo = np.uint64(0xFFFFFFFF)
+    i4 = np.asarray(i4, np.uint64)
+    x = [i4 & lo, i4 >> np.uint64(32), np.full_like(i4, step & 0xFFFFFFFF), np.full_like(i4, (step >> 32) & 0xFFFFFFFF)]
+    k = [seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF]
+    for _ in range(rounds):
+        p, q = x[0] * np.uint64(0xD2511F53), x[2] * np.uint64(0xCD9E8D57)
+        x = [(q >> np.uint64(32)) ^ x[1] ^ np.uint64(k[0]), q & lo, (p >> np.uint64(32)) ^ x[3] ^ np.uint64(k[1]), p & lo]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(x, 1)
+
+
+def dropout_kept(first, n, p, seed, step):
+    """bool [n]: elements first .. first + n - 1 that stay"""
+    i = np.arange(first, first + n, dtype=np.uint64)
+    groups = np.arange(first // 4, (first + n + 3) // 4, dtype=np.uint64)
+    words = philox4x32(groups, step, seed).reshape(-1)[first - 4 * (first // 4):][:n]
+    assert words.shape == i.shape
+    return words.astype(np.float64) >= np.floor(p * 2.0 ** 32 + 0.5)
+
+
+def dropout(x, p, seed, step=0, bias=None, relu=False):
+    """float64: relu?(kept ? (x + bias) / (1 - p) : 0)"""
+    kept = dropout_kept(0, x.size, p, seed, step).reshape(x.shape)
+    v = np.asarray(x, np.float64) + (0.0 if bias is None else np.asarray(bias, np.float64))
+    v = np.where(kept, v / (1.0 - p) if p < 1 else 0.0, 0.0)
+    return np.where(v < 0, 0.0, v) if relu else v
+
+
+def dropout_bwd(gy, p, seed, step=0, y=None):
+    """float64 (gradient w.r.t. x, w.r.t. bias)"""
+    kept = dropout_kept(0, gy.size, p, seed, step).reshape(gy.shape)
+    if y is not None:
+        kept = kept & ~(np.asarray(y, np.float64) <= 0)
+    g = np.where(kept, np.asarray(gy, np.float64) / (1.0 - p) if p < 1 else 0.0, 0.0)
+    return g, g.reshape(-1, g.shape[-1]).sum(0)
+
+
+MX4_GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def mx4_quantize(x):
+    """x [rows, cols] -> (codes [rows, cols] 0..15, scale bytes [rows, ceil(cols / 32)]) by comparison with the grid's midpoints, ties to the even
+    code, in float64 (exact: every input is a float of 32 bits or fewer)"""
+    rows, cols = x.shape
+    nb = -(-cols // 32)
+    b = np.zeros((rows, nb * 32))
+    b[:, :cols] = x
+    b = b.reshape(rows, nb, 32)
+    bad = ~np.isfinite(b).all(2)
+    b = np.where(bad[:, :, None], 0.0, b)
+    _, e = np.frexp(np.abs(b).max(2))
+    scale = np.where(np.abs(b).max(2) == 0, 0, np.clip(e - 1 - 2, -127, 127) + 127)
+    a = np.abs(np.ldexp(b, (127 - scale)[:, :, None].astype(np.int32)))
+    mid = (MX4_GRID[1:] + MX4_GRID[:-1]) / 2
+    code = np.zeros(a.shape, np.int64)
+    for k, m in enumerate(mid):                          # between code k and k + 1: the tie goes to the even one
+        code[(a > m) if k % 2 == 0 else (a >= m)] = k + 1
+    code = np.where(np.signbit(b), code + 8, code)
+    code[bad] = 0
+    return code.reshape(rows, -1)[:, :cols].astype(np.uint8), np.where(bad, 255, scale).astype(np.uint8)
+
+
+def mx4_dequantize(codes, scales):
+    cols = codes.shape[1]
+    unit = np.where(scales == 255, np.nan, np.ldexp(1.0, scales.astype(np.int32) - 127))
+    v = MX4_GRID[codes & 7] * np.where(codes & 8, -1.0, 1.0)
+    return v * np.repeat(unit, 32, 1)[:, :cols]
+
+
+def mx4_values(x):
+    """the values (float64) that x [rows, cols] takes when held in MXFP4"""
+    return mx4_dequantize(*mx4_quantize(x))
