@@ -140,11 +140,13 @@ SIGNATURES = {
     "adv_dropout_bwd": [_P, _P, _P, _P, _P, _L, _L, _I, _D, _U, _P, _L, _P],
     "adv_mx4_quantize": [_P, _P, _P, _L, _L, _I, _P],
     "adv_mx4_dequantize": [_P, _P, _P, _L, _L, _I, _P],
-    "adv_mx4_linear": [_P, _P, _P, _P, _P, _P, _L, _L, _L, _I, _I, _P],
-    "adv_mx4_linear_dgrad": [_P, _P, _P, _P, _P, _L, _L, _L, _I, _P],
+    "adv_mx4_linear": [_P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _I, _I, _P],
+    "adv_mx4_linear_dgrad": [_P, _P, _P, _P, _P, _P, _L, _L, _L, _I, _P],
 }
 _OTHER = {
     "adv_mx4_code_bytes": ([_L, _L], ctypes.c_int64),
+    "adv_mx4_linear_workspace_bytes": ([_L, _L, _L], ctypes.c_int64),
+    "adv_mx4_linear_dgrad_workspace_bytes": ([_L, _L, _L, _I], ctypes.c_int64),
     "adv_dropout_bwd_workspace_floats": ([_L, _L, _I], ctypes.c_int64),
     "adv_abi_version": ([], _I),
     "adv_build_has_test_hooks": ([], _I),

@@ -31,6 +31,21 @@ __device__ __forceinline__ void load_some(const T* p, float (&out)[V], int n) {
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = i < n ? static_cast<float>(p[i]) : 0.0f;
 }
+// eight elements, the first n of them real
+template <class T>
+__device__ __forceinline__ void load_eight(const T* p, float (&out)[8], int n) {
+  if (n < 8) {
+    load_some<T, 8>(p, out, n);
+  } else if constexpr (sizeof(T) == 2) {
+    load<T, 8>(p, out);
+  } else {
+    float a[4], b[4];
+    load<T, 4>(p, a);
+    load<T, 4>(p + 4, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = a[i], out[4 + i] = b[i];
+  }
+}
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
   static_assert(V * sizeof(T) == 16, "one 16-byte access");

@@ -27,6 +27,7 @@ constexpr int kPanel = 256;                // columns of a panel: 128 code bytes
 typedef int Int8 __attribute__((ext_vector_type(8)));
 typedef float Float16 __attribute__((ext_vector_type(16)));
 typedef float Float2 __attribute__((ext_vector_type(2)));
+typedef float Float4 __attribute__((ext_vector_type(4)));
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t Uint4 __attribute__((ext_vector_type(4)));
 
@@ -111,9 +112,10 @@ __global__ __launch_bounds__(kBlock) void mx4_dequantize(const uint8_t* __restri
   }
 }
 
-// ---- the product.  v_mfma_scale_f32_32x32x64_f8f6f4 with both operands e2m1: lane l holds 32 consecutive values of row l % 32 of A (or B), the
-//      first half of the wave the lower and the second the upper 32 of the 64, and their scale byte.  Which columns those are is free as long
-//      as A and B agree: here the lower half takes the first four blocks of a panel in turn, the upper half the last four.
+// ---- the product.  v_mfma_scale_f32_*_f8f6f4 with both operands e2m1: a lane holds 32 consecutive values of one row of A (or B) - one block -
+//      and that block's scale byte.  Which columns they are is free as long as A and B agree, so a lane takes neighbouring blocks of its row
+//      for successive instructions: its codes are one contiguous piece of the panel and its scale bytes one aligned word, whose byte the
+//      instruction selects.
 struct Operand {
   const uint8_t* codes;
   const uint8_t* scales;
@@ -124,54 +126,261 @@ __device__ __forceinline__ Int8 widen(Uint4 v) {
   return Int8{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0};
 }
 
-template <int SEL>
-__device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa, uint32_t sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(a), widen(b), c, 4, 4, SEL, static_cast<int>(sa), SEL, static_cast<int>(sb));
-}
-
 template <class T>
 __device__ __forceinline__ float finish(float v, const T* bias, int64_t n, int relu) {
   if (bias) v += static_cast<float>(bias[n]);
   return relu && v < 0.0f ? 0.0f : v;      // (a NaN stays)
 }
 
-// One 32 x 32 tile of y a workgroup, its four waves taking the panels in turn and joining their sums in LDS.
+// Workgroup ids are dealt to the eight XCDs in turn, each with its own L2: give neighbouring tiles to one XCD.  (A remainder of ids keeps its
+// place.)
+__device__ __forceinline__ int by_xcd(int id, int total) {
+  const int whole = total & ~7;
+  return id < whole ? (id & 7) * (whole >> 3) + (id >> 3) : id;
+}
+
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+// Asks for ROWS 128-byte rows to be copied straight into LDS (16 bytes a lane, lanes in order), swizzled by taking chunk c ^ (row % 8) to place c.
+// ``at``: this lane's byte offset in the source for each of the ROWS / 32 requests of a thread.
+template <int ROWS>
+__device__ __forceinline__ void stage(const void* base, uint32_t bytes, const uint32_t (&at)[ROWS / 32], uint8_t* lds, int wave) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
+#pragma unroll
+  for (int j = 0; j < ROWS / 32; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + j * 4096 + wave * 1024), 16, static_cast<int>(at[j]), 0, 0, 0);
+}
+
+// 16-byte chunk c of a 128-byte row r lies at chunk c ^ (r % 8): eight rows' equal chunks are in eight different places
+__device__ __forceinline__ int swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// Where a workgroup stores its tile: a resource over the tile's real rows (row pitch ``pitch`` bytes), so that rows behind the last one are dropped by
+// its range check; a column behind the last one is given kNowhere.
+constexpr uint32_t kNowhere = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(void* base, int64_t m0, int64_t rows, int bm, int64_t pitch) {
+  const int64_t bytes = min(static_cast<int64_t>(bm), rows - m0) * pitch;
+  return __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(base) + m0 * pitch, 0, static_cast<int>(bytes), 0x00020000);
+}
 template <class T>
-__global__ __launch_bounds__(kBlock) void mx4_linear(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y, int64_t panels, int relu) {
-  __shared__ float s_sum[3][16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 32, n0 = static_cast<int64_t>(blockIdx.x) * 32;
-  const int64_t m = min(m0 + (lane & 31), x.rows - 1), n = min(n0 + (lane & 31), w.rows - 1);      // rows behind the last one are computed, not stored
-  Float16 acc = {};
-  for (int64_t p = wave; p < panels; p += 4) {
-    const Uint4* xa = reinterpret_cast<const Uint4*>(x.codes + (p * x.rows + m) * 128 + half * 64);
-    const Uint4* wb = reinterpret_cast<const Uint4*>(w.codes + (p * w.rows + n) * 128 + half * 64);
-    const uint32_t sx = *reinterpret_cast<const uint32_t*>(x.scales + (p * x.rows + m) * 8 + half * 4);
-    const uint32_t sw = *reinterpret_cast<const uint32_t*>(w.scales + (p * w.rows + n) * 8 + half * 4);
-    acc = mfma<0>(xa[0], wb[0], acc, sx, sw);
-    acc = mfma<1>(xa[1], wb[1], acc, sx, sw);
-    acc = mfma<2>(xa[2], wb[2], acc, sx, sw);
-    acc = mfma<3>(xa[3], wb[3], acc, sx, sw);
-  }
-  if (wave > 0) {
+__device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t to, uint32_t at, float v) {
+  if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), to, static_cast<int>(at), 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, static_cast<T>(v)), to, static_cast<int>(at), 0, 0);
+}
+// One 32 x 32 accumulator: lane l holds column l % 32, rows 8 (e / 4) + 4 (l / 32) + e % 4
+template <class T>
+__device__ __forceinline__ void put_tile(__amdgpu_buffer_rsrc_t to, const Float16& acc, int row, int half, int64_t col, int64_t cols, float bias, int relu) {
+  const uint32_t pitch = static_cast<uint32_t>(cols * sizeof(T)), at = col < cols ? static_cast<uint32_t>(row + 4 * half) * pitch + static_cast<uint32_t>(col * sizeof(T)) : kNowhere;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_sum[wave - 1][i][lane] = acc[i];
-  }
-  __syncthreads();
-  if (wave > 0) return;
-  const int64_t nn = n0 + (lane & 31);
-  if (nn >= w.rows) return;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t mm = m0 + 8 * (i / 4) + 4 * half + i % 4;
-    const float v = acc[i] + s_sum[0][i][lane] + s_sum[1][i][lane] + s_sum[2][i][lane];
-    if (mm < x.rows) y[mm * w.rows + nn] = static_cast<T>(finish<T>(v, bias, nn, relu));
+  for (int e = 0; e < 16; ++e) {
+    float v = acc[e] + bias;
+    if (relu && v < 0.0f) v = 0.0f;                    // (a NaN stays)
+    put<T>(to, at == kNowhere ? at : at + (8 * (e / 4) + e % 4) * pitch, v);
   }
 }
 
-// ---- the input gradient.  A workgroup owns kGradRows rows x one panel of gx and walks W's rows 64 at a time: their codes become bfloat16
-//      values in LDS, turned so that a lane's eight values along the contraction are 16 bytes; gy goes there as its bfloat16 terms.
-constexpr int kGradRows = 64, kChunk = 64;
+// Few rows of x: bound by reading W once.  16 rows of W (A) x 16 * MT rows of x (B) a workgroup on 16x16x128 instructions, operands straight
+// from memory to registers (a panel's 16 rows are 2 KB in one piece); the waves share the panels out and join their sums in LDS, in order.
+template <class T, int MT>
+__global__ __launch_bounds__(1024) void mx4_linear_thin(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y, int panels, int relu) {
+  extern __shared__ __attribute__((aligned(16))) float s_sum[];        // [wave][MT][4][64]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, quarter = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
+  const int64_t n = min(n0 + (lane & 15), w.rows - 1);                 // rows behind the last one are computed, not stored
+  int64_t m[MT];
+  Float4 acc[MT] = {};
+#pragma unroll
+  for (int i = 0; i < MT; ++i) m[i] = min(m0 + 16 * i + (lane & 15), x.rows - 1);
+  constexpr int U = MT == 1 ? 4 : 2;                                   // panels whose operands are on their way together
+  for (int p0 = wave; p0 < panels; p0 += waves * U) {
+    Uint4 a[U][2], b[U][MT][2];
+    uint32_t sa[U], sb[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t p = min(p0 + u * waves, panels - 1);
+      const Uint4* at = reinterpret_cast<const Uint4*>(w.codes + (p * w.rows + n) * 128 + quarter * 32);
+      a[u][0] = at[0], a[u][1] = at[1];
+      sa[u] = *reinterpret_cast<const uint16_t*>(w.scales + (p * w.rows + n) * 8 + quarter * 2);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const Uint4* bt = reinterpret_cast<const Uint4*>(x.codes + (p * x.rows + m[i]) * 128 + quarter * 32);
+        b[u][i][0] = bt[0], b[u][i][1] = bt[1];
+        sb[u][i] = *reinterpret_cast<const uint16_t*>(x.scales + (p * x.rows + m[i]) * 8 + quarter * 2);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u * waves < panels) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(a[u][0]), widen(b[u][i][0]), acc[i], 4, 4, 0, static_cast<int>(sa[u]), 0,
+                                                                    static_cast<int>(sb[u][i]));
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(a[u][1]), widen(b[u][i][1]), acc[i], 4, 4, 1, static_cast<int>(sa[u]), 1,
+                                                                    static_cast<int>(sb[u][i]));
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_sum[((wave * MT + i) * 4 + e) * 64 + lane] = acc[i][e];
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 256; o += blockDim.x) {           // (m, n) of the tile, n fastest; a lane held row n = 4 (lane / 16) + e, column m = lane % 16
+    const int i = o >> 8, mm = (o >> 4) & 15, nn = o & 15;
+    const int at = (i * 4 + (nn & 3)) * 64 + (nn >> 2) * 16 + mm;
+    float v = s_sum[at];
+    for (int k = 1; k < waves; ++k) v += s_sum[k * MT * 256 + at];
+    if (m0 + 16 * i + mm < x.rows && n0 + nn < w.rows) y[(m0 + 16 * i + mm) * w.rows + n0 + nn] = static_cast<T>(finish<T>(v, bias, n0 + nn, relu));
+  }
+}
+
+template <int SEL>
+__device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(a), widen(b), c, 4, 4, SEL, static_cast<int>(sa), SEL, static_cast<int>(sb));
+}
+
+// Many rows: BM x BN of y a workgroup of four waves (2 x 2), 32x32x64 instructions; panels go to LDS by direct copies, two buffers, one barrier a
+// panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is multiplied, and the barrier stands before
+// a panel's last step, whose operands are in registers by then - its products cover the first reads of the next panel.
+// The order of a step's instructions: a wave issues in order and a matrix instruction holds the next one back for its 32 cycles, so what else the
+// step has to issue - READS of LDS, COPIES into it - goes one by one (copies two) behind its PRODUCTS instead of before them.
+template <int READS, int COPIES, int PRODUCTS>
+__device__ __forceinline__ void weave() {
+#pragma unroll
+  for (int k = 0; k < PRODUCTS; ++k) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (k < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    else if (2 * (k - READS) < COPIES) __builtin_amdgcn_sched_group_barrier(0x010, 2, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int BM, int BN>
+constexpr int kTileLds = 2 * (BM + BN) * 128;
+
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y,
+                                                                               float* __restrict__ partial, int panels, int splits, int relu) {
+  constexpr int TM = BM / 64, TN = BN / 64, kStage = (BM + BN) * 128;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_tile[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int tm = static_cast<int>((x.rows + BM - 1) / BM), tn = static_cast<int>((w.rows + BN - 1) / BN);
+  int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+  const int part = id / (tm * tn);
+  id -= part * tm * tn;
+  const int group = 4 * tn, first = id / group * 4, high = min(4, tm - first);      // four rows of tiles at a time: both operands stay in the L2
+  const int64_t m0 = static_cast<int64_t>(first + id % group % high) * BM, n0 = static_cast<int64_t>(id % group / high) * BN;
+  const int begin = static_cast<int>(static_cast<int64_t>(part) * panels / splits), end = static_cast<int>(static_cast<int64_t>(part + 1) * panels / splits);
+
+  uint32_t at_x[BM / 32], at_w[BN / 32];
+  const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4;
+#pragma unroll
+  for (int j = 0; j < BM / 32; ++j) at_x[j] = static_cast<uint32_t>(min(m0 + j * 32 + wave * 8 + (lane >> 3), x.rows - 1)) * 128u + chunk;
+#pragma unroll
+  for (int j = 0; j < BN / 32; ++j) at_w[j] = static_cast<uint32_t>(min(n0 + j * 32 + wave * 8 + (lane >> 3), w.rows - 1)) * 128u + chunk;
+  const uint32_t x_bytes = static_cast<uint32_t>(x.rows) * 128u, w_bytes = static_cast<uint32_t>(w.rows) * 128u;
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+  uint32_t row_x[TM], row_w[TN];                       // byte offsets of this lane's scale words in a panel
+#pragma unroll
+  for (int i = 0; i < TM; ++i) row_x[i] = static_cast<uint32_t>(min(m0 + wm + i * 32 + (lane & 31), x.rows - 1)) * 8u + half * 4;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) row_w[j] = static_cast<uint32_t>(min(n0 + wn + j * 32 + (lane & 31), w.rows - 1)) * 8u + half * 4;
+  int frag[4];                                         // this lane's chunk of a row in each of the four steps
+#pragma unroll
+  for (int k = 0; k < 4; ++k) frag[k] = swizzled(lane & 31, half * 4 + k);
+
+  auto request = [&](int p, int buf) {
+    stage<BM>(x.codes + static_cast<int64_t>(p) * x_bytes, x_bytes, at_x, s_tile + buf * kStage, wave);
+    stage<BN>(w.codes + static_cast<int64_t>(p) * w_bytes, w_bytes, at_w, s_tile + buf * kStage + BM * 128, wave);
+  };
+  Uint4 fa[2][TM], fb[2][TN];
+  auto read = [&](int buf, int k, int to) {
+    const uint8_t* a = s_tile + buf * kStage + wm * 128 + frag[k];
+    const uint8_t* b = s_tile + buf * kStage + (BM + wn) * 128 + frag[k];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[to][i] = *reinterpret_cast<const Uint4*>(a + i * 4096);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[to][j] = *reinterpret_cast<const Uint4*>(b + j * 4096);
+  };
+  uint32_t sx[TM], sw[TN], nx[TM], nw[TN];
+  auto scale_words = [&](int p, uint32_t (&ox)[TM], uint32_t (&ow)[TN]) {
+    const uint8_t* a = x.scales + static_cast<int64_t>(p) * x.rows * 8;
+    const uint8_t* b = w.scales + static_cast<int64_t>(p) * w.rows * 8;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ox[i] = *reinterpret_cast<const uint32_t*>(a + row_x[i]);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) ow[j] = *reinterpret_cast<const uint32_t*>(b + row_w[j]);
+  };
+  Float16 acc[TM][TN] = {};
+#define MX4_STEP(SEL, FROM)                                                                             \
+  _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j)        \
+      acc[i][j] = mfma<SEL>(fa[FROM][i], fb[FROM][j], acc[i][j], sx[i], sw[j])
+
+  // (the tail's requests beyond the last panel ask for that one again, into the buffer nobody reads: one loop body, no branches)
+  const int last = end - 1;
+  request(begin, 0);
+  scale_words(begin, sx, sw);
+  request(min(begin + 1, last), 1);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  read(0, 0, 0);
+  int buf = 0;
+  for (int p = begin; p < end; ++p) {
+    read(buf, 1, 1);
+    MX4_STEP(0, 0);
+    weave<TM + TN, 0, TM * TN>();
+    scale_words(min(p + 1, last), nx, nw);
+    read(buf, 2, 0);
+    MX4_STEP(1, 1);
+    weave<TM + TN, 0, TM * TN>();
+    read(buf, 3, 1);
+    MX4_STEP(2, 0);
+    weave<TM + TN, 0, TM * TN>();
+    // every wave has this panel's operands in registers, and its copies of the next panel have landed
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    request(min(p + 2, last), buf);
+    buf ^= 1;
+    read(buf, 0, 0);
+    MX4_STEP(3, 1);
+    weave<TM + TN, (BM + BN) / 32, TM * TN>();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) sx[i] = nx[i];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sw[j] = nw[j];
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // no copy may land in an LDS that is another workgroup's by then
+#undef MX4_STEP
+  float* to = partial + static_cast<int64_t>(part) * x.rows * w.rows;
+  const __amdgpu_buffer_rsrc_t out = splits > 1 ? tile_rows(to, m0, x.rows, BM, w.rows * 4) : tile_rows(y, m0, x.rows, BM, w.rows * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int64_t n = n0 + wn + j * 32 + (lane & 31);
+    const float b = bias && splits == 1 ? static_cast<float>(bias[min(n, w.rows - 1)]) : 0.0f;
+    if (splits > 1) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) put_tile<float>(out, acc[i][j], wm + i * 32, half, n, w.rows, 0.0f, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) put_tile<T>(out, acc[i][j], wm + i * 32, half, n, w.rows, b, relu);
+    }
+  }
+}
+
+// y = relu?(part 0 + part 1 + ... + bias), in that order
+template <class T>
+__global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ partial, const T* __restrict__ bias, T* __restrict__ y, int64_t n, int64_t cols,
+                                                   int parts, int relu) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    float v = partial[i];
+    for (int k = 1; k < parts; ++k) v += partial[k * n + i];
+    y[i] = static_cast<T>(finish<T>(v, bias, bias ? i % cols : 0, relu));
+  }
+}
+
+// ---- the input gradient.  First gy, 0 where the ReLU stopped it, becomes planes of bfloat16 terms [term][row][n padded to 64] - once, not in
+//      every workgroup that needs it.  Then a workgroup owns BM rows x one panel of gx and walks W's rows 64 at a time: their codes become
+//      bfloat16 values in LDS, turned so that a lane's eight values along the contraction are 16 bytes; the terms are copied there.
+constexpr int kChunk = 64;
 
 template <class T>
 constexpr int kTerms = sizeof(T) == 4 ? 3 : 2;
@@ -191,116 +400,134 @@ __device__ __forceinline__ void split(float v, uint32_t (&t)[N]) {
   }
 }
 
-// 16-byte chunk c of a 128-byte row r lies at chunk c ^ (r % 8): eight rows' equal chunks are in eight different places
-__device__ __forceinline__ int swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
-
+// a thread: eight consecutive n of a row
 template <class T>
-__global__ __launch_bounds__(kBlock) void mx4_dgrad(const T* __restrict__ gy, const T* __restrict__ mask, Operand w, T* __restrict__ gx, int64_t rows,
-                                                    int64_t cols) {
+__global__ __launch_bounds__(kBlock) void mx4_grad_terms(const T* __restrict__ gy, const T* __restrict__ mask, uint8_t* __restrict__ planes, int64_t rows, int64_t n,
+                                                         int64_t padded) {
   constexpr int N = kTerms<T>;
-  __shared__ __attribute__((aligned(16))) uint8_t s_w[kPanel * 128];
-  __shared__ __attribute__((aligned(16))) uint8_t s_g[N][kGradRows * 128];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
-  const int64_t panel = blockIdx.x, m0 = static_cast<int64_t>(blockIdx.y) * kGradRows, nw = w.rows;
-  Float16 acc[2][2] = {};
-  for (int64_t n0 = 0; n0 < nw; n0 += kChunk) {
-    __syncthreads();
-    {  // eight rows (n) x eight columns of W a thread
-      const int o = t & 7, u = t >> 3;
-      uint32_t q[8];
-      float unit[8];
+  const int64_t per_row = padded / 8, unit = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  if (unit >= rows * per_row) return;
+  const int64_t m = unit / per_row, c = (unit - m * per_row) * 8;
+  const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(8), n - c)));
+  float g[8], o[8];
+  lowp::load_eight<T>(gy + m * n + c, g, left);
+  if (mask) {
+    lowp::load_eight<T>(mask + m * n + c, o, left);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t n = n0 + 8 * o + j;
-        const bool in = n < nw;
-        const int64_t at = panel * nw + (in ? n : nw - 1);
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(w.codes + at * 128 + 4 * u);
-        const uint32_t scale = w.scales[at * 8 + u / 4];
-        q[j] = in ? code : 0u;
-        unit[j] = __uint_as_float((in ? scale : 127u) << 23);
-      }
-      uint32_t v[8][4];                      // [row][pair of columns]
+    for (int k = 0; k < 8; ++k) g[k] = o[k] <= 0.0f ? 0.0f : g[k];
+  }
+  Uint4 out[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], unit[j], 0));
-        v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], unit[j], 1));
-        v[j][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], unit[j], 2));
-        v[j][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], unit[j], 3));
-      }
+  for (int k = 0; k < 4; ++k) {
+    uint32_t a[N], b[N];
+    split<N>(g[2 * k], a);
+    split<N>(g[2 * k + 1], b);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {          // column 8u + k: its eight rows' values
-        Uint4 out;
+    for (int s = 0; s < N; ++s) out[s][k] = a[s] | b[s] << 16;
+  }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t a = v[2 * j][k / 2], b = v[2 * j + 1][k / 2];
-          out[j] = k & 1 ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
-        }
-        *reinterpret_cast<Uint4*>(s_w + swizzled(8 * u + k, o)) = out;
-      }
+  for (int s = 0; s < N; ++s) *reinterpret_cast<Uint4*>(planes + ((s * rows + m) * padded + c) * 2) = out[s];
+}
+
+template <int N, int BM>
+constexpr int kGradLds = (kPanel + N * BM) * 128;
+
+template <class T, int BM>
+__global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial, int64_t rows,
+                                                       int64_t cols, int64_t padded, int splits) {
+  constexpr int N = kTerms<T>, WM = BM == 128 ? 2 : 1, WK = 4 / WM, TI = BM / WM / 32, TJ = kPanel / WK / 32;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_grad[];
+  uint8_t* s_w = s_grad;
+  uint8_t* s_g = s_grad + kPanel * 128;                // [term][BM rows][128 bytes]
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
+  const int tiles_m = static_cast<int>((rows + BM - 1) / BM), panels = static_cast<int>(panels_of(cols));
+  int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+  const int part = id / (tiles_m * panels);
+  id -= part * tiles_m * panels;
+  const int64_t panel = id / tiles_m, m0 = static_cast<int64_t>(id % tiles_m) * BM, nw = w.rows;
+  const int chunks = static_cast<int>(padded / kChunk);
+  const int begin = static_cast<int>(static_cast<int64_t>(part) * chunks / splits), end = static_cast<int>(static_cast<int64_t>(part + 1) * chunks / splits);
+  const int wm = wave / WK * (TI * 32), wk = wave % WK * (TJ * 32);
+
+  uint32_t at[BM / 32];
+#pragma unroll
+  for (int j = 0; j < BM / 32; ++j)
+    at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(j * 32 + wave * 8 + (lane >> 3)), rows - 1 - m0) * padded * 2) + (static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4);
+  const uint8_t* plane0 = planes + m0 * padded * 2;
+  const uint32_t tile_bytes = static_cast<uint32_t>(min(static_cast<int64_t>(BM), rows - m0) * padded * 2);
+
+  // eight rows (n) x eight columns of W a thread
+  const int o = t & 7, u = t >> 3;
+  uint32_t q[8], unit[8];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t n = static_cast<int64_t>(c) * kChunk + 8 * o + j;
+      const bool in = n < nw;
+      const int64_t row = panel * nw + (in ? n : nw - 1);
+      const uint32_t code = *reinterpret_cast<const uint32_t*>(w.codes + row * 128 + 4 * u);
+      const uint32_t scale = w.scales[row * 8 + u / 4];
+      q[j] = in ? code : 0u;                           // (rows behind the last one meet zero terms: they must not be NaN)
+      unit[j] = in ? scale : 127u;
     }
-    for (int unit = t; unit < kGradRows * (kChunk / 8); unit += kBlock) {      // eight consecutive n of a row of gy
-      const int r = unit >> 3, c = unit & 7;
-      const int64_t m = m0 + r, n = n0 + 8 * c;
-      float g[8];
+  };
+  Float16 acc[TI][TJ] = {};
+  fetch(begin);
+  for (int c = begin; c < end; ++c) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = 0.0f;
-      if (m < rows) {
-        const T* p = gy + m * nw + n;
-        const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(8), nw - n)));
-        lowp::load_some<T, 8>(p, g, left);
-        if (mask) {
-          float o[8];
-          lowp::load_some<T, 8>(mask + m * nw + n, o, left);
+    for (int s = 0; s < N; ++s)
+      stage<BM>(plane0 + s * rows * padded * 2 + static_cast<int64_t>(c) * (kChunk * 2), tile_bytes - static_cast<uint32_t>(c) * (kChunk * 2), at, s_g + s * BM * 128, wave);
+    uint32_t v[8][4];                                  // [row][pair of columns]
 #pragma unroll
-          for (int k = 0; k < 8; ++k) g[k] = o[k] <= 0.0f ? 0.0f : g[k];
-        }
-      }
-      Uint4 out[N];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t a[N], b[N];
-        split<N>(g[2 * k], a);
-        split<N>(g[2 * k + 1], b);
-#pragma unroll
-        for (int s = 0; s < N; ++s) out[s][k] = a[s] | b[s] << 16;
-      }
-#pragma unroll
-      for (int s = 0; s < N; ++s) *reinterpret_cast<Uint4*>(s_g[s] + swizzled(r, c)) = out[s];
+    for (int j = 0; j < 8; ++j) {
+      const float f = __uint_as_float(unit[j] << 23);
+      v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 0));
+      v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 1));
+      v[j][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 2));
+      v[j][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 3));
     }
-    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kChunk / 16; ++k) {  // 16 of the contraction a matrix instruction: lane half h has chunk 2k + h
-      Bf16x8 b[2];
+    for (int k = 0; k < 8; ++k) {                      // column 8u + k: its eight rows' values
+      Uint4 out;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(s_w + swizzled(wave * 64 + j * 32 + (lane & 31), 2 * k + half));
+      for (int j = 0; j < 4; ++j) out[j] = __builtin_amdgcn_perm(v[2 * j + 1][k / 2], v[2 * j][k / 2], k & 1 ? 0x07060302u : 0x05040100u);
+      *reinterpret_cast<Uint4*>(s_w + swizzled(8 * u + k, o)) = out;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch(min(c + 1, end - 1));
+#pragma unroll
+    for (int k = 0; k < kChunk / 16; ++k) {            // 16 of the contraction a matrix instruction: lane half h has chunk 2k + h
+      Bf16x8 b[TJ];
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(s_w + swizzled(wk + j * 32 + (lane & 31), 2 * k + half));
 #pragma unroll
       for (int s = 0; s < N; ++s) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(s_g[s] + swizzled(i * 32 + (lane & 31), 2 * k + half));
+        for (int i = 0; i < TI; ++i) {
+          const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(s_g + s * BM * 128 + swizzled(wm + i * 32 + (lane & 31), 2 * k + half));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
         }
       }
     }
   }
+  float* to = partial + static_cast<int64_t>(part) * rows * cols;
+  const __amdgpu_buffer_rsrc_t out = splits > 1 ? tile_rows(to, m0, rows, BM, cols * 4) : tile_rows(gx, m0, rows, BM, cols * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int j = 0; j < TJ; ++j) {
+    const int64_t col = panel * kPanel + wk + j * 32 + (lane & 31);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t col = panel * kPanel + wave * 64 + j * 32 + (lane & 31);
-      if (col >= cols) continue;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t m = m0 + i * 32 + 8 * (e / 4) + 4 * half + e % 4;
-        if (m < rows) gx[m * cols + col] = static_cast<T>(acc[i][j][e]);
-      }
+    for (int i = 0; i < TI; ++i) {
+      if (splits > 1) put_tile<float>(out, acc[i][j], wm + i * 32, half, col, cols, 0.0f, 0);
+      else put_tile<T>(out, acc[i][j], wm + i * 32, half, col, cols, 0.0f, 0);
     }
   }
 }
 
 // sizes: every product of two of them fits an int64, every grid dimension its limit
-constexpr int64_t kMostRows = int64_t{1} << 20, kMostCols = int64_t{1} << 22;
+constexpr int64_t kMostRows = int64_t{1} << 20, kMostCols = int64_t{1} << 20;      // 256 rows of a result: at most 2^30 bytes
 
 bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 1 && cols >= 1 && rows <= kMostRows && cols <= kMostCols; }
 int64_t code_bytes(int64_t rows, int64_t cols) { return panels_of(cols) * rows * (kPanel / 2); }
@@ -322,17 +549,105 @@ int run_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int64_t
   mx4_dequantize<T><<<panel_grid<T>(rows, cols), kBlock, 0, st>>>(codes, scales, static_cast<T*>(x), rows, cols);
   return adv_internal_finish_launch();
 }
+constexpr int64_t kAlign = 256;
+int64_t padded(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
+
+// How a product is cut: thin tiles up to 64 rows; above, 256 x 256 tiles where they fill half the chip, else 128 x 128, the panels dealt to
+// several workgroups a tile where tiles alone do not fill it (at least four panels each: a workgroup's start and the joining pass cost about two).
+struct LinearPlan {
+  int thin, big, splits;
+};
+LinearPlan plan_linear(int64_t m, int64_t n, int64_t k) {
+  const int64_t panels = panels_of(k);
+  if (m <= 64) return {1, 0, 1};
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
+  const bool use_big = big >= 128;
+  const int64_t tiles = use_big ? big : small, room = use_big ? 256 : 512;
+  int64_t s = room / tiles;
+  if (s > panels / 4) s = panels / 4;
+  if (s < 1) s = 1;
+  return {0, use_big ? 1 : 0, static_cast<int>(s)};
+}
+int64_t linear_partial_bytes(int64_t m, int64_t n, int64_t k) {
+  const LinearPlan p = plan_linear(m, n, k);
+  return p.splits > 1 ? padded(4LL * p.splits * m * n) : 0;
+}
+
 template <class T>
-int run_linear(Operand x, Operand w, const void* bias, void* y, int64_t k, int relu, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((w.rows + 31) / 32), static_cast<unsigned>((x.rows + 31) / 32));
-  mx4_linear<T><<<grid, kBlock, 0, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), panels_of(k), relu);
+void run_join(const float* partial, const void* bias, void* y, int64_t rows, int64_t cols, int parts, int relu, hipStream_t st) {
+  const int64_t n = rows * cols, blocks = (n + kBlock - 1) / kBlock;
+  mx4_join<T><<<dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), kBlock, 0, st>>>(partial, static_cast<const T*>(bias), static_cast<T*>(y), n, cols, parts,
+                                                                                         relu);
+}
+
+template <class T, int MT>
+int run_thin(Operand x, Operand w, const void* bias, void* y, int panels, int relu, hipStream_t st) {
+  const int waves = panels >= 16 ? 16 : (panels >= 4 ? 4 : 1), lds = waves * MT * 1024;
+  const dim3 grid(static_cast<unsigned>((w.rows + 15) / 16), static_cast<unsigned>((x.rows + 16 * MT - 1) / (16 * MT)));
+  if (!adv_internal_lds_limit<mx4_linear_thin<T, MT>>(16 * MT * 1024)) return ADV_ELAUNCH;
+  mx4_linear_thin<T, MT><<<grid, waves * 64, lds, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), panels, relu);
   return adv_internal_finish_launch();
 }
-template <class T>
-int run_dgrad(const void* gy, const void* mask, Operand w, void* gx, int64_t m, int64_t k, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(panels_of(k)), static_cast<unsigned>((m + kGradRows - 1) / kGradRows));
-  mx4_dgrad<T><<<grid, kBlock, 0, st>>>(static_cast<const T*>(gy), static_cast<const T*>(mask), w, static_cast<T*>(gx), m, k);
+
+template <class T, int BM, int BN>
+int run_tile(Operand x, Operand w, const void* bias, void* y, float* partial, int panels, int splits, int relu, hipStream_t st) {
+  const int64_t tiles = ((x.rows + BM - 1) / BM) * ((w.rows + BN - 1) / BN) * splits;
+  if (!adv_internal_lds_limit<mx4_linear_tile<T, BM, BN>>(kTileLds<BM, BN>)) return ADV_ELAUNCH;
+  mx4_linear_tile<T, BM, BN><<<dim3(static_cast<unsigned>(tiles)), kBlock, kTileLds<BM, BN>, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), partial, panels,
+                                                                                                  splits, relu);
+  if (splits > 1) run_join<T>(partial, bias, y, x.rows, w.rows, splits, relu, st);
   return adv_internal_finish_launch();
+}
+
+template <class T>
+int run_linear(Operand x, Operand w, const void* bias, void* y, float* partial, int64_t k, int relu, hipStream_t st) {
+  const LinearPlan p = plan_linear(x.rows, w.rows, k);
+  const int panels = static_cast<int>(panels_of(k));
+  if (p.thin) {
+    if (x.rows <= 16) return run_thin<T, 1>(x, w, bias, y, panels, relu, st);
+    if (x.rows <= 32) return run_thin<T, 2>(x, w, bias, y, panels, relu, st);
+    return run_thin<T, 4>(x, w, bias, y, panels, relu, st);
+  }
+  if (p.big) return run_tile<T, 256, 256>(x, w, bias, y, partial, panels, p.splits, relu, st);
+  return run_tile<T, 128, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
+}
+
+// The input gradient: the contraction is dealt to several workgroups where panels x row tiles do not fill two workgroups a CU
+struct GradPlan {
+  int bm, splits;
+  int64_t padded_n;
+};
+GradPlan plan_dgrad(int64_t m, int64_t n, int64_t k) {
+  const int bm = m <= 32 ? 32 : (m <= 64 ? 64 : 128);
+  const int64_t chunks = (n + kChunk - 1) / kChunk, tiles = panels_of(k) * ((m + bm - 1) / bm);
+  int64_t s = 512 / tiles;
+  if (s > chunks / 4) s = chunks / 4;
+  if (s < 1) s = 1;
+  return {bm, static_cast<int>(s), chunks * kChunk};
+}
+int terms_of(int dtype) { return dtype == ADV_F32 ? 3 : (dtype == ADV_F16 ? 2 : 1); }
+int64_t plane_bytes(int64_t m, int64_t n, int dtype) { return padded(terms_of(dtype) * m * ((n + kChunk - 1) / kChunk * kChunk) * 2); }
+
+template <class T, int BM>
+int run_dgrad_tile(const uint8_t* planes, Operand w, void* gx, float* partial, int64_t m, int64_t k, const GradPlan& p, hipStream_t st) {
+  const int64_t blocks = panels_of(k) * ((m + BM - 1) / BM) * p.splits;
+  constexpr int lds = kGradLds<kTerms<T>, BM>;
+  if (!adv_internal_lds_limit<mx4_dgrad<T, BM>>(lds)) return ADV_ELAUNCH;
+  mx4_dgrad<T, BM><<<dim3(static_cast<unsigned>(blocks)), kBlock, lds, st>>>(planes, w, static_cast<T*>(gx), partial, m, k, p.padded_n, p.splits);
+  if (p.splits > 1) run_join<T>(partial, nullptr, gx, m, k, p.splits, 0, st);
+  return adv_internal_finish_launch();
+}
+
+template <class T>
+int run_dgrad(const void* gy, const void* mask, Operand w, void* gx, uint8_t* ws, int64_t m, int64_t k, int dtype, hipStream_t st) {
+  const GradPlan p = plan_dgrad(m, w.rows, k);
+  const int64_t units = m * (p.padded_n / 8);
+  mx4_grad_terms<T><<<dim3(static_cast<unsigned>((units + kBlock - 1) / kBlock)), kBlock, 0, st>>>(static_cast<const T*>(gy), static_cast<const T*>(mask), ws, m, w.rows,
+                                                                                                p.padded_n);
+  float* partial = reinterpret_cast<float*>(ws + plane_bytes(m, w.rows, dtype));
+  if (p.bm == 32) return run_dgrad_tile<T, 32>(ws, w, gx, partial, m, k, p, st);
+  if (p.bm == 64) return run_dgrad_tile<T, 64>(ws, w, gx, partial, m, k, p, st);
+  return run_dgrad_tile<T, 128>(ws, w, gx, partial, m, k, p, st);
 }
 
 }  // namespace
@@ -368,38 +683,65 @@ int adv_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int
   return run_dequantize<_Float16>(codes, scales, x, rows, cols, st);
 }
 
-int adv_mx4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias, void* y, int64_t m,
-                   int64_t n, int64_t k, int dtype, int relu, adv_stream_t stream) {
-  if (!x_codes || !x_scales || !w_codes || !w_scales || !y || !sizes_ok(m, k) || !sizes_ok(n, k) || !lowp::known(dtype)) return ADV_EINVAL;
-  const int e = lowp::size_of(dtype);
-  if (!lowp::aligned(x_codes, 16) || !lowp::aligned(w_codes, 16) || !lowp::aligned(x_scales, 8) || !lowp::aligned(w_scales, 8) || !lowp::aligned(y, e) ||
-      !lowp::aligned(bias, e))
-    return ADV_EALIGN;
-  const int64_t yb = m * n * e;
-  if (lowp::overlap(y, yb, x_codes, code_bytes(m, k)) || lowp::overlap(y, yb, x_scales, scale_bytes(m, k)) || lowp::overlap(y, yb, w_codes, code_bytes(n, k)) ||
-      lowp::overlap(y, yb, w_scales, scale_bytes(n, k)) || (bias && lowp::overlap(y, yb, bias, n * e)))
-    return ADV_EINVAL;
-  const Operand x{x_codes, x_scales, m}, w{w_codes, w_scales, n};
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ADV_F32) return run_linear<float>(x, w, bias, y, k, relu, st);
-  if (dtype == ADV_BF16) return run_linear<__bf16>(x, w, bias, y, k, relu, st);
-  return run_linear<_Float16>(x, w, bias, y, k, relu, st);
+int64_t adv_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  if (!sizes_ok(m, k) || !sizes_ok(n, k)) return ADV_EINVAL;
+  return padded(code_bytes(m, k)) + padded(scale_bytes(m, k)) + linear_partial_bytes(m, n, k);
 }
 
-int adv_mx4_linear_dgrad(const void* gy, const void* mask, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, int64_t m, int64_t n, int64_t k, int dtype,
-                         adv_stream_t stream) {
-  if (!gy || !w_codes || !w_scales || !gx || !sizes_ok(m, k) || !sizes_ok(n, k) || !lowp::known(dtype)) return ADV_EINVAL;
+int adv_mx4_linear(const void* x, const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias, void* y,
+                   void* workspace, int64_t m, int64_t n, int64_t k, int dtype, int relu, adv_stream_t stream) {
+  if (!w_codes || !w_scales || !y || !workspace || !sizes_ok(m, k) || !sizes_ok(n, k) || !lowp::known(dtype)) return ADV_EINVAL;
+  if (x ? (x_codes || x_scales) : (!x_codes || !x_scales)) return ADV_EINVAL;
   const int e = lowp::size_of(dtype);
-  if (!lowp::aligned(gy, e) || !lowp::aligned(mask, e) || !lowp::aligned(gx, e) || !lowp::aligned(w_codes, 16) || !lowp::aligned(w_scales, 8)) return ADV_EALIGN;
-  const int64_t xb = m * k * e, gb = m * n * e;
-  if (lowp::overlap(gx, xb, gy, gb) || (mask && lowp::overlap(gx, xb, mask, gb)) || lowp::overlap(gx, xb, w_codes, code_bytes(n, k)) ||
-      lowp::overlap(gx, xb, w_scales, scale_bytes(n, k)))
-    return ADV_EINVAL;
+  if (!lowp::aligned(x_codes, 16) || !lowp::aligned(w_codes, 16) || !lowp::aligned(x_scales, 8) || !lowp::aligned(w_scales, 8) || !lowp::aligned(y, e) ||
+      !lowp::aligned(bias, e) || !lowp::aligned(x, e) || !lowp::aligned(workspace, kAlign))
+    return ADV_EALIGN;
+  const struct { const void* at; int64_t bytes; } in[] = {{x, m * k * e}, {x_codes, code_bytes(m, k)}, {x_scales, scale_bytes(m, k)}, {w_codes, code_bytes(n, k)},
+                                                          {w_scales, scale_bytes(n, k)}, {bias, n * e}};
+  const int64_t yb = m * n * e, wb = adv_mx4_linear_workspace_bytes(m, n, k);
+  if (lowp::overlap(y, yb, workspace, wb)) return ADV_EINVAL;
+  for (const auto& b : in)
+    if (b.at && (lowp::overlap(y, yb, b.at, b.bytes) || lowp::overlap(workspace, wb, b.at, b.bytes))) return ADV_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (x) {
+    uint8_t* scales = ws + padded(code_bytes(m, k));
+    const int bad = dtype == ADV_F32 ? run_quantize<float>(x, ws, scales, m, k, st)
+                                     : (dtype == ADV_BF16 ? run_quantize<__bf16>(x, ws, scales, m, k, st) : run_quantize<_Float16>(x, ws, scales, m, k, st));
+    if (bad) return bad;
+    x_codes = ws, x_scales = scales;
+  }
+  float* partial = reinterpret_cast<float*>(ws + padded(code_bytes(m, k)) + padded(scale_bytes(m, k)));
+  const Operand xo{x_codes, x_scales, m}, wo{w_codes, w_scales, n};
+  if (dtype == ADV_F32) return run_linear<float>(xo, wo, bias, y, partial, k, relu, st);
+  if (dtype == ADV_BF16) return run_linear<__bf16>(xo, wo, bias, y, partial, k, relu, st);
+  return run_linear<_Float16>(xo, wo, bias, y, partial, k, relu, st);
+}
+
+int64_t adv_mx4_linear_dgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (!sizes_ok(m, k) || !sizes_ok(n, k) || !lowp::known(dtype)) return ADV_EINVAL;
+  const GradPlan p = plan_dgrad(m, n, k);
+  return plane_bytes(m, n, dtype) + (p.splits > 1 ? padded(4LL * p.splits * m * k) : 0);
+}
+
+int adv_mx4_linear_dgrad(const void* gy, const void* mask, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, void* workspace, int64_t m, int64_t n, int64_t k,
+                         int dtype, adv_stream_t stream) {
+  if (!gy || !w_codes || !w_scales || !gx || !workspace || !sizes_ok(m, k) || !sizes_ok(n, k) || !lowp::known(dtype)) return ADV_EINVAL;
+  const int e = lowp::size_of(dtype);
+  if (!lowp::aligned(gy, e) || !lowp::aligned(mask, e) || !lowp::aligned(gx, e) || !lowp::aligned(w_codes, 16) || !lowp::aligned(w_scales, 8) ||
+      !lowp::aligned(workspace, kAlign))
+    return ADV_EALIGN;
+  const struct { const void* at; int64_t bytes; } in[] = {{gy, m * n * e}, {mask, m * n * e}, {w_codes, code_bytes(n, k)}, {w_scales, scale_bytes(n, k)}};
+  const int64_t xb = m * k * e, wb = adv_mx4_linear_dgrad_workspace_bytes(m, n, k, dtype);
+  if (lowp::overlap(gx, xb, workspace, wb)) return ADV_EINVAL;
+  for (const auto& b : in)
+    if (b.at && (lowp::overlap(gx, xb, b.at, b.bytes) || lowp::overlap(workspace, wb, b.at, b.bytes))) return ADV_EINVAL;
   const Operand w{w_codes, w_scales, n};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == ADV_F32) return run_dgrad<float>(gy, mask, w, gx, m, k, st);
-  if (dtype == ADV_BF16) return run_dgrad<__bf16>(gy, mask, w, gx, m, k, st);
-  return run_dgrad<_Float16>(gy, mask, w, gx, m, k, st);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (dtype == ADV_F32) return run_dgrad<float>(gy, mask, w, gx, ws, m, k, dtype, st);
+  if (dtype == ADV_BF16) return run_dgrad<__bf16>(gy, mask, w, gx, ws, m, k, dtype, st);
+  return run_dgrad<_Float16>(gy, mask, w, gx, ws, m, k, dtype, st);
 }
 
 }  // extern "C"

@@ -103,10 +103,13 @@ def mx4_linear(x, w, bias=None, relu=False, dtype=None):
         raise ValueError("bias must be [%d], got %s" % (w.rows, tuple(bias.shape)))
     if not y.numel():
         return y
-    q = _mx4(x, "x") if isinstance(x, Mx4) else mx4_quantize(x)
+    held = _mx4(x, "x") if isinstance(x, Mx4) else None
+    m = y.numel() // w.rows
     with _on(y):
-        _lib.call("adv_mx4_linear", q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-                  None if bias is None else bias.data_ptr(), y.data_ptr(), q.rows, w.rows, w.cols, _FLOATS[dtype], 1 if relu else 0, _stream(y))
+        ws = torch.empty((_lib.load().adv_mx4_linear_workspace_bytes(m, w.rows, w.cols),), dtype=torch.uint8, device=y.device)
+        _lib.call("adv_mx4_linear", x.data_ptr() if held is None else None, None if held is None else held.codes.data_ptr(),
+                  None if held is None else held.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                  y.data_ptr(), ws.data_ptr(), m, w.rows, w.cols, _FLOATS[dtype], 1 if relu else 0, _stream(y))
     return y
 
 
@@ -126,9 +129,11 @@ def mx4_linear_dgrad(grad_y, w, mask=None):
         return gx
     if not w.rows:
         return gx.zero_()
+    m, kind = gx.numel() // w.cols, _FLOATS[gx.dtype]
     with _on(gx):
+        ws = torch.empty((_lib.load().adv_mx4_linear_dgrad_workspace_bytes(m, w.rows, w.cols, kind),), dtype=torch.uint8, device=gx.device)
         _lib.call("adv_mx4_linear_dgrad", grad_y.data_ptr(), None if mask is None else mask.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gx.data_ptr(),
-                  gx.numel() // w.cols, w.rows, w.cols, _FLOATS[gx.dtype], _stream(gx))
+                  ws.data_ptr(), m, w.rows, w.cols, kind, _stream(gx))
     return gx
 
 

@@ -650,19 +650,24 @@ ADV_API int adv_dropout_bwd(const void* gy, const void* y, void* gx, void* gbias
 /* Matrices held in MXFP4: 32 consecutive values of a row as 4-bit floats (e2m1) under one power of two (e8m0).
  *     codes   [panels][rows][128] bytes, panels = ceil(cols / 256), the value of an even column in the low nibble; 16-byte aligned,
  *             adv_mx4_code_bytes bytes.  scales [panels][rows][8] bytes (a sixteenth of that), 8-byte aligned.  Columns behind `cols` are zero.
- *     rows <= 2^20, cols <= 2^22.
+ *     rows <= 2^20, cols <= 2^20.
  *   _quantize   per block e = clamp(floor(log2 max|x|) - 2, -127, 127), codes nearest-even(x / 2^e) saturated at 6, scale byte e + 127; a block that
  *               holds a NaN or an infinity gets scale byte 255: it is NaN as a whole.
- *   _linear     y [m, n] = relu?(X . W^T + bias) for X [m, k] and W [n, k] in MXFP4, bias [n] or NULL; products exact, sums float32.
+ *   _linear     y [m, n] = relu?(X . W^T + bias) for X [m, k] and W [n, k] in MXFP4, bias [n] or NULL; products exact, sums float32.  X comes as
+ *               values x [m, k] of type `dtype` (then x_codes = x_scales = NULL: quantised on the way), or as x_codes / x_scales (then x = NULL).
  *   _linear_dgrad  gx [m, k] = G . W, G [m, n] = gy, 0 where mask (NULL, or laid out like gy: the layer's ReLU output) is <= 0; gy enters exactly,
- *               sums float32. */
+ *               sums float32.
+ *   workspace   device memory of _workspace_bytes bytes, 256-byte aligned, not shared with a call that may run at the same time.
+ *   The order of the additions depends on the sizes alone: the same call gives the same bits. */
 ADV_API int64_t adv_mx4_code_bytes(int64_t rows, int64_t cols);
 ADV_API int adv_mx4_quantize(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, int dtype, adv_stream_t stream);
 ADV_API int adv_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int64_t cols, int dtype, adv_stream_t stream);
-ADV_API int adv_mx4_linear(const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias, void* y,
-                           int64_t m, int64_t n, int64_t k, int dtype, int relu, adv_stream_t stream);
-ADV_API int adv_mx4_linear_dgrad(const void* gy, const void* mask, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, int64_t m, int64_t n,
-                                 int64_t k, int dtype, adv_stream_t stream);
+ADV_API int64_t adv_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+ADV_API int adv_mx4_linear(const void* x, const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
+                           void* y, void* workspace, int64_t m, int64_t n, int64_t k, int dtype, int relu, adv_stream_t stream);
+ADV_API int64_t adv_mx4_linear_dgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype);
+ADV_API int adv_mx4_linear_dgrad(const void* gy, const void* mask, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, void* workspace, int64_t m,
+                                 int64_t n, int64_t k, int dtype, adv_stream_t stream);
 
 #ifdef __cplusplus
 }
