@@ -243,25 +243,27 @@ __device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa
 // panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is multiplied, and the barrier stands before
 // a panel's last step, whose operands are in registers by then - its products cover the first reads of the next panel.
 // The order of a step's instructions: a wave issues in order and a matrix instruction holds the next one back for its 32 cycles, so what else the
-// step has to issue - READS of LDS, COPIES into it - goes one by one (copies two) behind its PRODUCTS instead of before them.
+// step has to issue - READS of LDS, COPIES into it - goes behind its PRODUCTS one by one instead of before them.
 template <int READS, int COPIES, int PRODUCTS>
 __device__ __forceinline__ void weave() {
+  constexpr int kReads = (2 * READS + PRODUCTS - 1) / PRODUCTS, kCopies = (COPIES + PRODUCTS - 1) / PRODUCTS;      // behind one product; reads within the first half
 #pragma unroll
   for (int k = 0; k < PRODUCTS; ++k) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if (k < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    else if (2 * (k - READS) < COPIES) __builtin_amdgcn_sched_group_barrier(0x010, 2, 0);
+    if (k * kReads < READS) __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    if (k * kCopies < COPIES) __builtin_amdgcn_sched_group_barrier(0x010, kCopies, 0);
   }
   __builtin_amdgcn_sched_barrier(0);
 }
 
+constexpr int kAhead = 3;                  // panels between a line's first touch and its copy to LDS: a line nobody has asked for yet is 2 us away
 template <int BM, int BN>
-constexpr int kTileLds = 2 * (BM + BN) * 128;
+constexpr int kTileLds = 2 * (BM + BN) * (128 + 8) + 2048;
 
 template <class T, int BM, int BN>
 __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y,
                                                                                float* __restrict__ partial, int panels, int splits, int relu) {
-  constexpr int TM = BM / 64, TN = BN / 64, kStage = (BM + BN) * 128;
+  constexpr int TM = BM / 64, TN = BN / 64, kStage = (BM + BN) * (128 + 8), kScales = (BM + BN) * 128;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_tile[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int tm = static_cast<int>((x.rows + BM - 1) / BM), tn = static_cast<int>((w.rows + BN - 1) / BN);
@@ -280,18 +282,31 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   for (int j = 0; j < BN / 32; ++j) at_w[j] = static_cast<uint32_t>(min(n0 + j * 32 + wave * 8 + (lane >> 3), w.rows - 1)) * 128u + chunk;
   const uint32_t x_bytes = static_cast<uint32_t>(x.rows) * 128u, w_bytes = static_cast<uint32_t>(w.rows) * 128u;
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-  uint32_t row_x[TM], row_w[TN];                       // byte offsets of this lane's scale words in a panel
-#pragma unroll
-  for (int i = 0; i < TM; ++i) row_x[i] = static_cast<uint32_t>(min(m0 + wm + i * 32 + (lane & 31), x.rows - 1)) * 8u + half * 4;
-#pragma unroll
-  for (int j = 0; j < TN; ++j) row_w[j] = static_cast<uint32_t>(min(n0 + wn + j * 32 + (lane & 31), w.rows - 1)) * 8u + half * 4;
   int frag[4];                                         // this lane's chunk of a row in each of the four steps
 #pragma unroll
   for (int k = 0; k < 4; ++k) frag[k] = swizzled(lane & 31, half * 4 + k);
 
+  // the tile's scale bytes of a panel are one piece of BM (BN) * 8 bytes: 1 KB a wave (128 x 128 tiles have two: two waves copy each)
+  const int piece = wave % ((BM + BN) / 128);
+  const bool for_x = piece < BM / 128;
+  const uint32_t at_scale = static_cast<uint32_t>((for_x ? m0 + piece * 128 : n0 + (piece - BM / 128) * 128) * 8) + lane * 16;
+  const int to_scale = kScales + piece * 1024;
+  const uint8_t* scales = for_x ? x.scales : w.scales;
+  const uint32_t scale_bytes = (for_x ? x_bytes : w_bytes) >> 4;
+  const uint32_t touched = static_cast<uint32_t>(min(m0 + threadIdx.x % BM, x.rows - 1)) * 128u, touched_w = static_cast<uint32_t>(min(n0 + threadIdx.x % BN, w.rows - 1)) * 128u;
   auto request = [&](int p, int buf) {
-    stage<BM>(x.codes + static_cast<int64_t>(p) * x_bytes, x_bytes, at_x, s_tile + buf * kStage, wave);
-    stage<BN>(w.codes + static_cast<int64_t>(p) * w_bytes, w_bytes, at_w, s_tile + buf * kStage + BM * 128, wave);
+    const int64_t q = p;
+    stage<BM>(x.codes + q * x_bytes, x_bytes, at_x, s_tile + buf * kStage, wave);
+    stage<BN>(w.codes + q * w_bytes, w_bytes, at_w, s_tile + buf * kStage + BM * 128, wave);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales + q * scale_bytes), 0, static_cast<int>(scale_bytes), 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(s_tile + buf * kStage + to_scale), 16, static_cast<int>(at_scale), 0, 0, 0);
+  };
+  auto touch = [&](int p) {
+    const int64_t q = p;
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x.codes + q * x_bytes), 0, static_cast<int>(x_bytes), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w.codes + q * w_bytes), 0, static_cast<int>(w_bytes), 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (LdsVoid*)(s_tile + 2 * kStage + wave * 512), 4, static_cast<int>(touched), 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (LdsVoid*)(s_tile + 2 * kStage + wave * 512 + 256), 4, static_cast<int>(touched_w), 0, 0, 0);
   };
   Uint4 fa[2][TM], fb[2][TN];
   auto read = [&](int buf, int k, int to) {
@@ -302,51 +317,55 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[to][j] = *reinterpret_cast<const Uint4*>(b + j * 4096);
   };
-  uint32_t sx[TM], sw[TN], nx[TM], nw[TN];
-  auto scale_words = [&](int p, uint32_t (&ox)[TM], uint32_t (&ow)[TN]) {
-    const uint8_t* a = x.scales + static_cast<int64_t>(p) * x.rows * 8;
-    const uint8_t* b = w.scales + static_cast<int64_t>(p) * w.rows * 8;
+  uint32_t sx[2][TM], sw[2][TN];
+  auto scale_words = [&](int buf, int to) {
+    const uint8_t* a = s_tile + buf * kStage + kScales + (wm + (lane & 31)) * 8 + half * 4;
+    const uint8_t* b = s_tile + buf * kStage + kScales + (BM + wn + (lane & 31)) * 8 + half * 4;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) ox[i] = *reinterpret_cast<const uint32_t*>(a + row_x[i]);
+    for (int i = 0; i < TM; ++i) sx[to][i] = *reinterpret_cast<const uint32_t*>(a + i * 256);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) ow[j] = *reinterpret_cast<const uint32_t*>(b + row_w[j]);
+    for (int j = 0; j < TN; ++j) sw[to][j] = *reinterpret_cast<const uint32_t*>(b + j * 256);
   };
   Float16 acc[TM][TN] = {};
 #define MX4_STEP(SEL, FROM)                                                                             \
   _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j)        \
-      acc[i][j] = mfma<SEL>(fa[FROM][i], fb[FROM][j], acc[i][j], sx[i], sw[j])
+      acc[i][j] = mfma<SEL>(fa[FROM][i], fb[FROM][j], acc[i][j], sx[0][i], sw[0][j])
 
   // (the tail's requests beyond the last panel ask for that one again, into the buffer nobody reads: one loop body, no branches)
   const int last = end - 1;
   request(begin, 0);
-  scale_words(begin, sx, sw);
   request(min(begin + 1, last), 1);
+#pragma unroll
+  for (int k = 2; k < kAhead + 2; ++k) touch(min(begin + k, last));
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
   read(0, 0, 0);
+  scale_words(0, 0);
   int buf = 0;
   for (int p = begin; p < end; ++p) {
     read(buf, 1, 1);
     MX4_STEP(0, 0);
     weave<TM + TN, 0, TM * TN>();
-    scale_words(min(p + 1, last), nx, nw);
     read(buf, 2, 0);
     MX4_STEP(1, 1);
     weave<TM + TN, 0, TM * TN>();
     read(buf, 3, 1);
     MX4_STEP(2, 0);
     weave<TM + TN, 0, TM * TN>();
-    // every wave has this panel's operands in registers, and its copies of the next panel have landed
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // every wave has this panel's operands in registers, and its copies of the next panel have landed (the two lines touched after them may
+    // still be on their way)
+    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     request(min(p + 2, last), buf);
+    touch(min(p + 2 + kAhead, last));
     buf ^= 1;
     read(buf, 0, 0);
+    scale_words(buf, 1);
     MX4_STEP(3, 1);
-    weave<TM + TN, (BM + BN) / 32, TM * TN>();
+    weave<2 * (TM + TN), (BM + BN) / 32 + 3, TM * TN>();
 #pragma unroll
-    for (int i = 0; i < TM; ++i) sx[i] = nx[i];
+    for (int i = 0; i < TM; ++i) sx[0][i] = sx[1][i];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sw[j] = nw[j];
+    for (int j = 0; j < TN; ++j) sw[0][j] = sw[1][j];
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // no copy may land in an LDS that is another workgroup's by then
 #undef MX4_STEP
