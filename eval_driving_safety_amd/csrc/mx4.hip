@@ -141,7 +141,7 @@ __device__ __forceinline__ int by_xcd(int id, int total) {
 
 typedef __attribute__((address_space(3))) void LdsVoid;
 
-// Asks for ROWS 128-byte rows to be copied straight into LDS (16 bytes a lane, lanes in order), swizzled by taking chunk c ^ (row % 8) to place c.
+// Asks for ROWS 128-byte rows to be copied straight into LDS (16 bytes a lane, lanes in order), swizzled: see staged_chunk.
 // ``at``: this lane's byte offset in the source for each of the ROWS / 32 requests of a thread.
 template <int ROWS>
 __device__ __forceinline__ void stage(const void* base, uint32_t bytes, const uint32_t (&at)[ROWS / 32], uint8_t* lds, int wave) {
@@ -150,8 +150,11 @@ __device__ __forceinline__ void stage(const void* base, uint32_t bytes, const ui
   for (int j = 0; j < ROWS / 32; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + j * 4096 + wave * 1024), 16, static_cast<int>(at[j]), 0, 0, 0);
 }
 
-// 16-byte chunk c of a 128-byte row r lies at chunk c ^ (r % 8): eight rows' equal chunks are in eight different places
-__device__ __forceinline__ int swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+// 16-byte chunk c of a 128-byte row r lies at chunk c ^ (r / 2 % 8): two rows fill the 64 banks, so the equal chunks of any sixteen neighbouring
+// rows - what a 16-byte read serves at a time - are in sixteen different places
+__device__ __forceinline__ int swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row >> 1 & 7)) << 4); }
+// the chunk that lane ``lane`` of wave ``wave`` fetches so that it lands there (rows of a request: 8 * wave + lane / 8, plus multiples of 32)
+__device__ __forceinline__ uint32_t staged_chunk(int wave, int lane) { return static_cast<uint32_t>((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7)) << 4; }
 
 // Where a workgroup stores its tile: a resource over the tile's real rows (row pitch ``pitch`` bytes), so that rows behind the last one are dropped by
 // its range check; a column behind the last one is given kNowhere.
@@ -256,9 +259,8 @@ __device__ __forceinline__ void weave() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-constexpr int kAhead = 3;                  // panels between a line's first touch and its copy to LDS: a line nobody has asked for yet is 2 us away
 template <int BM, int BN>
-constexpr int kTileLds = 2 * (BM + BN) * (128 + 8) + 2048;
+constexpr int kTileLds = 2 * (BM + BN) * (128 + 8);
 
 template <class T, int BM, int BN>
 __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y,
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   const int begin = static_cast<int>(static_cast<int64_t>(part) * panels / splits), end = static_cast<int>(static_cast<int64_t>(part + 1) * panels / splits);
 
   uint32_t at_x[BM / 32], at_w[BN / 32];
-  const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4;
+  const uint32_t chunk = staged_chunk(wave, lane);
 #pragma unroll
   for (int j = 0; j < BM / 32; ++j) at_x[j] = static_cast<uint32_t>(min(m0 + j * 32 + wave * 8 + (lane >> 3), x.rows - 1)) * 128u + chunk;
 #pragma unroll
@@ -293,20 +295,12 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   const int to_scale = kScales + piece * 1024;
   const uint8_t* scales = for_x ? x.scales : w.scales;
   const uint32_t scale_bytes = (for_x ? x_bytes : w_bytes) >> 4;
-  const uint32_t touched = static_cast<uint32_t>(min(m0 + threadIdx.x % BM, x.rows - 1)) * 128u, touched_w = static_cast<uint32_t>(min(n0 + threadIdx.x % BN, w.rows - 1)) * 128u;
   auto request = [&](int p, int buf) {
     const int64_t q = p;
     stage<BM>(x.codes + q * x_bytes, x_bytes, at_x, s_tile + buf * kStage, wave);
     stage<BN>(w.codes + q * w_bytes, w_bytes, at_w, s_tile + buf * kStage + BM * 128, wave);
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales + q * scale_bytes), 0, static_cast<int>(scale_bytes), 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(s_tile + buf * kStage + to_scale), 16, static_cast<int>(at_scale), 0, 0, 0);
-  };
-  auto touch = [&](int p) {
-    const int64_t q = p;
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x.codes + q * x_bytes), 0, static_cast<int>(x_bytes), 0x00020000);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w.codes + q * w_bytes), 0, static_cast<int>(w_bytes), 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (LdsVoid*)(s_tile + 2 * kStage + wave * 512), 4, static_cast<int>(touched), 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (LdsVoid*)(s_tile + 2 * kStage + wave * 512 + 256), 4, static_cast<int>(touched_w), 0, 0, 0);
   };
   Uint4 fa[2][TM], fb[2][TN];
   auto read = [&](int buf, int k, int to) {
@@ -335,8 +329,6 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   const int last = end - 1;
   request(begin, 0);
   request(min(begin + 1, last), 1);
-#pragma unroll
-  for (int k = 2; k < kAhead + 2; ++k) touch(min(begin + k, last));
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
   read(0, 0, 0);
   scale_words(0, 0);
@@ -351,17 +343,15 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
     read(buf, 3, 1);
     MX4_STEP(2, 0);
     weave<TM + TN, 0, TM * TN>();
-    // every wave has this panel's operands in registers, and its copies of the next panel have landed (the two lines touched after them may
-    // still be on their way)
-    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // every wave has this panel's operands in registers, and its copies of the next panel have landed
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     request(min(p + 2, last), buf);
-    touch(min(p + 2 + kAhead, last));
     buf ^= 1;
     read(buf, 0, 0);
     scale_words(buf, 1);
     MX4_STEP(3, 1);
-    weave<2 * (TM + TN), (BM + BN) / 32 + 3, TM * TN>();
+    weave<2 * (TM + TN), (BM + BN) / 32 + 1, TM * TN>();
 #pragma unroll
     for (int i = 0; i < TM; ++i) sx[0][i] = sx[1][i];
 #pragma unroll
@@ -451,6 +441,10 @@ __global__ __launch_bounds__(kBlock) void mx4_grad_terms(const T* __restrict__ g
 template <int N, int BM>
 constexpr int kGradLds = (kPanel + N * BM) * 128;
 
+// the LDS row of a column: every other group of eight has its neighbours swapped, so that the rows which sixteen lanes write together (eight columns
+// apart) lie in both halves of the banks
+__device__ __forceinline__ int turned(int col) { return col ^ (col >> 3 & 1); }
+
 template <class T, int BM>
 __global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial, int64_t rows,
                                                        int64_t cols, int64_t padded, int splits) {
@@ -471,7 +465,7 @@ __global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict
   uint32_t at[BM / 32];
 #pragma unroll
   for (int j = 0; j < BM / 32; ++j)
-    at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(j * 32 + wave * 8 + (lane >> 3)), rows - 1 - m0) * padded * 2) + (static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4);
+    at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(j * 32 + wave * 8 + (lane >> 3)), rows - 1 - m0) * padded * 2) + staged_chunk(wave, lane);
   const uint8_t* plane0 = planes + m0 * padded * 2;
   const uint32_t tile_bytes = static_cast<uint32_t>(min(static_cast<int64_t>(BM), rows - m0) * padded * 2);
 
@@ -511,7 +505,7 @@ __global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict
       Uint4 out;
 #pragma unroll
       for (int j = 0; j < 4; ++j) out[j] = __builtin_amdgcn_perm(v[2 * j + 1][k / 2], v[2 * j][k / 2], k & 1 ? 0x07060302u : 0x05040100u);
-      *reinterpret_cast<Uint4*>(s_w + swizzled(8 * u + k, o)) = out;
+      *reinterpret_cast<Uint4*>(s_w + swizzled(turned(8 * u + k), o)) = out;
     }
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -520,7 +514,7 @@ __global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict
     for (int k = 0; k < kChunk / 16; ++k) {            // 16 of the contraction a matrix instruction: lane half h has chunk 2k + h
       Bf16x8 b[TJ];
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(s_w + swizzled(wk + j * 32 + (lane & 31), 2 * k + half));
+      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(s_w + swizzled(turned(wk + j * 32 + (lane & 31)), 2 * k + half));
 #pragma unroll
       for (int s = 0; s < N; ++s) {
 #pragma unroll
