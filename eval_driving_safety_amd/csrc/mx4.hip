@@ -29,6 +29,7 @@ typedef float Float16 __attribute__((ext_vector_type(16)));
 typedef float Float2 __attribute__((ext_vector_type(2)));
 typedef float Float4 __attribute__((ext_vector_type(4)));
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t Uint2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Uint4 __attribute__((ext_vector_type(4)));
 
 __host__ __device__ inline int64_t panels_of(int64_t cols) { return (cols + kPanel - 1) / kPanel; }
@@ -387,9 +388,9 @@ __global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ par
 }
 
 // ---- the input gradient.  First gy, 0 where the ReLU stopped it, becomes planes of bfloat16 terms [term][row][n padded to 64] - once, not in
-//      every workgroup that needs it.  Then a workgroup owns BM rows x one panel of gx and walks W's rows 64 at a time: their codes become
+//      every workgroup that needs it.  Then a workgroup owns BM rows x one panel of gx and walks W's rows 32 at a time: their codes become
 //      bfloat16 values in LDS, turned so that a lane's eight values along the contraction are 16 bytes; the terms are copied there.
-constexpr int kChunk = 64;
+constexpr int kChunk = 32;
 
 template <class T>
 constexpr int kTerms = sizeof(T) == 4 ? 3 : 2;
@@ -438,94 +439,139 @@ __global__ __launch_bounds__(kBlock) void mx4_grad_terms(const T* __restrict__ g
   for (int s = 0; s < N; ++s) *reinterpret_cast<Uint4*>(planes + ((s * rows + m) * padded + c) * 2) = out[s];
 }
 
+// Rows of a stage are 64 bytes here (32 of the contraction): four of them fill the banks, so chunk c of row r lies at c ^ (r / 4 % 4), and the LDS row of
+// a column has its place in its group of four turned by the group of eight it belongs to - what the lanes of one write have, columns eight apart,
+// then falls into all four quarters of the banks.
+__device__ __forceinline__ int short_row(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
+__device__ __forceinline__ int turned(int col) { return col ^ (col >> 3 & 3); }
+
 template <int N, int BM>
-constexpr int kGradLds = (kPanel + N * BM) * 128;
+constexpr int kGradLds = 2 * (kPanel + N * BM) * 64;
 
-// the LDS row of a column: every other group of eight has its neighbours swapped, so that the rows which sixteen lanes write together (eight columns
-// apart) lie in both halves of the banks
-__device__ __forceinline__ int turned(int col) { return col ^ (col >> 3 & 1); }
-
+// Everything is doubled: while chunk c is multiplied, chunk c + 1 of W is taken from registers to LDS, the copies of its terms land, and chunks c + 2
+// and c + 3 of W are on their way to registers.  One barrier a chunk.
 template <class T, int BM>
-__global__ __launch_bounds__(kBlock, 2) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial, int64_t rows,
-                                                       int64_t cols, int64_t padded, int splits) {
+__global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial,
+                                                                      int64_t rows, int64_t cols, int64_t padded, int splits) {
   constexpr int N = kTerms<T>, WM = BM == 128 ? 2 : 1, WK = 4 / WM, TI = BM / WM / 32, TJ = kPanel / WK / 32;
-  extern __shared__ __attribute__((aligned(16))) uint8_t s_grad[];
-  uint8_t* s_w = s_grad;
-  uint8_t* s_g = s_grad + kPanel * 128;                // [term][BM rows][128 bytes]
+  constexpr int kCopies = BM >= 64 ? BM / 64 : 1, kTermBytes = BM * 64;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_grad[];      // [2][column][64 bytes], [2][term][row][64 bytes]
+  uint8_t* s_g = s_grad + 2 * kPanel * 64;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
   const int tiles_m = static_cast<int>((rows + BM - 1) / BM), panels = static_cast<int>(panels_of(cols));
   int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
   const int part = id / (tiles_m * panels);
   id -= part * tiles_m * panels;
   const int64_t panel = id / tiles_m, m0 = static_cast<int64_t>(id % tiles_m) * BM, nw = w.rows;
-  const int chunks = static_cast<int>(padded / kChunk);
-  const int begin = static_cast<int>(static_cast<int64_t>(part) * chunks / splits), end = static_cast<int>(static_cast<int64_t>(part + 1) * chunks / splits);
+  const int pairs = static_cast<int>(padded / (2 * kChunk));
+  const int begin = static_cast<int>(static_cast<int64_t>(part) * pairs / splits) * 2, end = static_cast<int>(static_cast<int64_t>(part + 1) * pairs / splits) * 2;
+  const int last = end - 1;
   const int wm = wave / WK * (TI * 32), wk = wave % WK * (TJ * 32);
 
-  uint32_t at[BM / 32];
+  // a copy request is 16 rows of 64 bytes a wave (with 32 rows two waves ask for each)
+  uint32_t at[kCopies];
 #pragma unroll
-  for (int j = 0; j < BM / 32; ++j)
-    at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(j * 32 + wave * 8 + (lane >> 3)), rows - 1 - m0) * padded * 2) + staged_chunk(wave, lane);
+  for (int j = 0; j < kCopies; ++j) {
+    const int row = j * 64 + (BM >= 64 ? wave : wave & 1) * 16 + (lane >> 2);
+    at[j] = static_cast<uint32_t>(min(static_cast<int64_t>(row), rows - 1 - m0) * padded * 2) + (static_cast<uint32_t>((lane & 3) ^ (row >> 2 & 3)) << 4);
+  }
   const uint8_t* plane0 = planes + m0 * padded * 2;
   const uint32_t tile_bytes = static_cast<uint32_t>(min(static_cast<int64_t>(BM), rows - m0) * padded * 2);
-
-  // eight rows (n) x eight columns of W a thread
-  const int o = t & 7, u = t >> 3;
-  uint32_t q[8], unit[8];
-  auto fetch = [&](int c) {
+  auto request = [&](int c, int buf) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t n = static_cast<int64_t>(c) * kChunk + 8 * o + j;
-      const bool in = n < nw;
-      const int64_t row = panel * nw + (in ? n : nw - 1);
-      const uint32_t code = *reinterpret_cast<const uint32_t*>(w.codes + row * 128 + 4 * u);
-      const uint32_t scale = w.scales[row * 8 + u / 4];
-      q[j] = in ? code : 0u;                           // (rows behind the last one meet zero terms: they must not be NaN)
-      unit[j] = in ? scale : 127u;
+    for (int s = 0; s < N; ++s) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(plane0 + s * rows * padded * 2 + static_cast<int64_t>(c) * (kChunk * 2)), 0,
+                                                                         static_cast<int>(tile_bytes - static_cast<uint32_t>(c) * (kChunk * 2)), 0x00020000);
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(s_g + (buf * N + s) * kTermBytes + j * 4096 + (BM >= 64 ? wave : wave & 1) * 1024), 16, static_cast<int>(at[j]), 0,
+                                                 0, 0);
+    }
+  };
+
+  // four rows (n) x eight columns of W a thread: n = 4o + j, columns 8u ..; rows behind the last one read as zeros (the resource ends there), which
+  // is the value 0 under the scale 2^-127
+  const int o = t & 7, u = t >> 3;
+  struct Held {
+    uint32_t code[4], scale[4];
+  };
+  const uint8_t* codes = w.codes + panel * nw * 128;
+  const uint8_t* scales = w.scales + panel * nw * 8;
+  const uint32_t at_code = static_cast<uint32_t>(o * 512 + u * 4), at_scale = static_cast<uint32_t>(o * 32 + u / 4);
+  const int slab = static_cast<int>(nw);
+  auto fetch = [&](int c, Held& h) {
+    const uint32_t left = max(slab - c * kChunk, 0);
+    const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes + static_cast<int64_t>(c) * (kChunk * 128)), 0, static_cast<int>(left * 128u), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales + static_cast<int64_t>(c) * (kChunk * 8)), 0, static_cast<int>(left * 8u), 0x00020000);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h.code[j] = __builtin_amdgcn_raw_buffer_load_b32(rc, static_cast<int>(at_code + j * 128), 0, 0);
+      h.scale[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, static_cast<int>(at_scale + j * 8), 0, 0);
+    }
+  };
+  // where a thread's 8 bytes of column 8u + k go: short_row(turned(8u + k), o / 2), half of a chunk - as the place of column 8u and what k changes
+  const uint32_t put_at = static_cast<uint32_t>(short_row(turned(8 * u), o >> 1) + (o & 1) * 8);
+  auto turn = [&](const Held& h, int buf) {
+    uint32_t v[4][4];                                  // [row][pair of columns]
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = __uint_as_float(h.scale[j] << 23);
+      v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 0));
+      v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 1));
+      v[j][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 2));
+      v[j][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 3));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {                      // column 8u + k: its four rows' values
+      const uint32_t pick = k & 1 ? 0x07060302u : 0x05040100u;
+      const Uint2 out = {__builtin_amdgcn_perm(v[1][k / 2], v[0][k / 2], pick), __builtin_amdgcn_perm(v[3][k / 2], v[2][k / 2], pick)};
+      *reinterpret_cast<Uint2*>(s_grad + (put_at ^ static_cast<uint32_t>(k * 64 + (k >> 2) * 16)) + buf * (kPanel * 64)) = out;
     }
   };
   Float16 acc[TI][TJ] = {};
-  fetch(begin);
-  for (int c = begin; c < end; ++c) {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-    for (int s = 0; s < N; ++s)
-      stage<BM>(plane0 + s * rows * padded * 2 + static_cast<int64_t>(c) * (kChunk * 2), tile_bytes - static_cast<uint32_t>(c) * (kChunk * 2), at, s_g + s * BM * 128, wave);
-    uint32_t v[8][4];                                  // [row][pair of columns]
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = __uint_as_float(unit[j] << 23);
-      v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 0));
-      v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 1));
-      v[j][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 2));
-      v[j][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[j], f, 3));
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                      // column 8u + k: its eight rows' values
-      Uint4 out;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[j] = __builtin_amdgcn_perm(v[2 * j + 1][k / 2], v[2 * j][k / 2], k & 1 ? 0x07060302u : 0x05040100u);
-      *reinterpret_cast<Uint4*>(s_w + swizzled(turned(8 * u + k), o)) = out;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    fetch(min(c + 1, end - 1));
+  const uint8_t* const read_w = s_grad + wk * 64;
+  const uint8_t* const read_g = s_g + wm * 64;
+  const uint32_t place_w = static_cast<uint32_t>(short_row(turned(lane & 31), half)), place_g = static_cast<uint32_t>(short_row(lane & 31, half));
+  auto multiply = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < kChunk / 16; ++k) {            // 16 of the contraction a matrix instruction: lane half h has chunk 2k + h
       Bf16x8 b[TJ];
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(s_w + swizzled(turned(wk + j * 32 + (lane & 31)), 2 * k + half));
+      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(read_w + (place_w ^ static_cast<uint32_t>(k * 32)) + buf * (kPanel * 64) + j * 2048);
 #pragma unroll
       for (int s = 0; s < N; ++s) {
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
-          const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(s_g + s * BM * 128 + swizzled(wm + i * 32 + (lane & 31), 2 * k + half));
+          const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(read_g + (place_g ^ static_cast<uint32_t>(k * 32)) + (buf * N + s) * kTermBytes + i * 2048);
 #pragma unroll
           for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
         }
       }
     }
+  };
+
+  Held h0, h1;
+  request(begin, 0);
+  __builtin_amdgcn_sched_barrier(0);                   // (the copies must be older than the eight loads that step() leaves on their way)
+  fetch(begin, h0);
+  fetch(min(begin + 1, last), h1);
+  turn(h0, 0);
+  fetch(min(begin + 2, last), h0);
+  // h: holds chunk c + 1, is given chunk c + 3
+  auto step = [&](int c, Held& h, int buf) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // chunk c's copies have landed: only the eight loads of chunk c + 2 came after
+    request(min(c + 1, last), buf ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    turn(h, buf ^ 1);
+    fetch(min(c + 3, last), h);
+    multiply(buf);
+  };
+  for (int c = begin; c < end; c += 2) {               // (chunks come in pairs: the planes are padded to them)
+    step(c, h1, 0);
+    step(c + 1, h0, 1);
   }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // no copy may land in an LDS that is another workgroup's by then
   float* to = partial + static_cast<int64_t>(part) * rows * cols;
   const __amdgpu_buffer_rsrc_t out = splits > 1 ? tile_rows(to, m0, rows, BM, cols * 4) : tile_rows(gx, m0, rows, BM, cols * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
@@ -632,14 +678,14 @@ struct GradPlan {
 };
 GradPlan plan_dgrad(int64_t m, int64_t n, int64_t k) {
   const int bm = m <= 32 ? 32 : (m <= 64 ? 64 : 128);
-  const int64_t chunks = (n + kChunk - 1) / kChunk, tiles = panels_of(k) * ((m + bm - 1) / bm);
-  int64_t s = 512 / tiles;
-  if (s > chunks / 4) s = chunks / 4;
+  const int64_t pairs = (n + 2 * kChunk - 1) / (2 * kChunk), tiles = panels_of(k) * ((m + bm - 1) / bm);
+  int64_t s = (bm == 128 ? 512 : 768) / tiles;
+  if (s > pairs / 4) s = pairs / 4;
   if (s < 1) s = 1;
-  return {bm, static_cast<int>(s), chunks * kChunk};
+  return {bm, static_cast<int>(s), pairs * 2 * kChunk};
 }
 int terms_of(int dtype) { return dtype == ADV_F32 ? 3 : (dtype == ADV_F16 ? 2 : 1); }
-int64_t plane_bytes(int64_t m, int64_t n, int dtype) { return padded(terms_of(dtype) * m * ((n + kChunk - 1) / kChunk * kChunk) * 2); }
+int64_t plane_bytes(int64_t m, int64_t n, int dtype) { return padded(terms_of(dtype) * m * plan_dgrad(m, n, 1).padded_n * 2); }
 
 template <class T, int BM>
 int run_dgrad_tile(const uint8_t* planes, Operand w, void* gx, float* partial, int64_t m, int64_t k, const GradPlan& p, hipStream_t st) {
