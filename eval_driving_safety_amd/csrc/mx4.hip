@@ -387,7 +387,7 @@ __global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ par
   }
 }
 
-// ---- the input gradient.  First gy, 0 where the ReLU stopped it, becomes planes of bfloat16 terms [term][row][n padded to 64] - once, not in
+// ---- the input gradient.  First gy, 0 where the ReLU stopped it, becomes planes of bfloat16 terms [term][row][n padded to 128] - once, not in
 //      every workgroup that needs it.  Then a workgroup owns BM rows x one panel of gx and walks W's rows 32 at a time: their codes become
 //      bfloat16 values in LDS, turned so that a lane's eight values along the contraction are 16 bytes; the terms are copied there.
 constexpr int kChunk = 32;
@@ -439,17 +439,26 @@ __global__ __launch_bounds__(kBlock) void mx4_grad_terms(const T* __restrict__ g
   for (int s = 0; s < N; ++s) *reinterpret_cast<Uint4*>(planes + ((s * rows + m) * padded + c) * 2) = out[s];
 }
 
-// Rows of a stage are 64 bytes here (32 of the contraction): four of them fill the banks, so chunk c of row r lies at c ^ (r / 4 % 4), and the LDS row of
-// a column has its place in its group of four turned by the group of eight it belongs to - what the lanes of one write have, columns eight apart,
-// then falls into all four quarters of the banks.
+// LDS places of a stage.  Terms: rows of 64 bytes (32 of the contraction); four of them fill the banks, so chunk c of row r lies at c ^ (r / 4 % 4).
+// W: rows (n) of 512 bytes (a panel's 256 columns), in units of 16 bytes; what is written together - two rows, eight blocks of columns, the same unit
+// of each - and what a transposing read takes together - four rows, four neighbouring units - must lie in different banks.
 __device__ __forceinline__ int short_row(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
-__device__ __forceinline__ int turned(int col) { return col ^ (col >> 3 & 3); }
+__device__ __forceinline__ int wide_row(int row, int unit) { return row * 512 + ((unit ^ (row & 3) << 2 ^ (unit >> 4 & 1) ^ (row & 1) << 1) << 4); }
+
+// ds_read_b64_tr_b16: sixteen lanes read 8 bytes each - lane 4r + s four columns of row r - and lane i gets column i of the four rows
+typedef __bf16 Bf16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Bf16x4 read_turned(const uint8_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) Bf16x4*)p);
+}
 
 template <int N, int BM>
 constexpr int kGradLds = 2 * (kPanel + N * BM) * 64;
 
-// Everything is doubled: while chunk c is multiplied, chunk c + 1 of W is taken from registers to LDS, the copies of its terms land, and chunks c + 2
-// and c + 3 of W are on their way to registers.  One barrier a chunk.
+// Everything is doubled: while chunk c is multiplied, chunk c + 1 of W is taken from registers to LDS, the copies of its terms land, and the next kHeld
+// chunks of W are on their way to registers (one 16-byte and one byte load a thread and chunk: what a load instruction costs hardly depends on its
+// width).  One barrier a chunk.  The matrix instruction wants eight n of one column in a lane; the codes come along the columns: they are stored as
+// bfloat16 rows and turned by the transposing LDS read.
+constexpr int kHeld = 4;
 template <class T, int BM>
 __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial,
                                                                       int64_t rows, int64_t cols, int64_t padded, int splits) {
@@ -463,8 +472,8 @@ __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uin
   const int part = id / (tiles_m * panels);
   id -= part * tiles_m * panels;
   const int64_t panel = id / tiles_m, m0 = static_cast<int64_t>(id % tiles_m) * BM, nw = w.rows;
-  const int pairs = static_cast<int>(padded / (2 * kChunk));
-  const int begin = static_cast<int>(static_cast<int64_t>(part) * pairs / splits) * 2, end = static_cast<int>(static_cast<int64_t>(part + 1) * pairs / splits) * 2;
+  const int fours = static_cast<int>(padded / (kHeld * kChunk));
+  const int begin = static_cast<int>(static_cast<int64_t>(part) * fours / splits) * kHeld, end = static_cast<int>(static_cast<int64_t>(part + 1) * fours / splits) * kHeld;
   const int last = end - 1;
   const int wm = wave / WK * (TI * 32), wk = wave % WK * (TJ * 32);
 
@@ -489,87 +498,89 @@ __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uin
     }
   };
 
-  // four rows (n) x eight columns of W a thread: n = 4o + j, columns 8u ..; rows behind the last one read as zeros (the resource ends there), which
-  // is the value 0 under the scale 2^-127
-  const int o = t & 7, u = t >> 3;
+  // 32 columns - one block - of one row of W a thread; rows behind the last one read as zeros (the resource ends there): the value 0 under the scale 2^-127
   struct Held {
-    uint32_t code[4], scale[4];
+    Uint4 code;
+    uint32_t scale;
   };
   const uint8_t* codes = w.codes + panel * nw * 128;
   const uint8_t* scales = w.scales + panel * nw * 8;
-  const uint32_t at_code = static_cast<uint32_t>(o * 512 + u * 4), at_scale = static_cast<uint32_t>(o * 32 + u / 4);
   const int slab = static_cast<int>(nw);
   auto fetch = [&](int c, Held& h) {
     const uint32_t left = max(slab - c * kChunk, 0);
     const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes + static_cast<int64_t>(c) * (kChunk * 128)), 0, static_cast<int>(left * 128u), 0x00020000);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales + static_cast<int64_t>(c) * (kChunk * 8)), 0, static_cast<int>(left * 8u), 0x00020000);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h.code[j] = __builtin_amdgcn_raw_buffer_load_b32(rc, static_cast<int>(at_code + j * 128), 0, 0);
-      h.scale[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, static_cast<int>(at_scale + j * 8), 0, 0);
-    }
+    h.code = __builtin_bit_cast(Uint4, __builtin_amdgcn_raw_buffer_load_b128(rc, t * 16, 0, 0));
+    h.scale = __builtin_amdgcn_raw_buffer_load_b8(rs, t, 0, 0);
   };
-  // where a thread's 8 bytes of column 8u + k go: short_row(turned(8u + k), o / 2), half of a chunk - as the place of column 8u and what k changes
-  const uint32_t put_at = static_cast<uint32_t>(short_row(turned(8 * u), o >> 1) + (o & 1) * 8);
+  const uint32_t put_at = static_cast<uint32_t>(wide_row(t >> 3, (t & 7) * 4));
   auto turn = [&](const Held& h, int buf) {
-    uint32_t v[4][4];                                  // [row][pair of columns]
+    const float f = __uint_as_float(h.scale << 23);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f = __uint_as_float(h.scale[j] << 23);
-      v[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 0));
-      v[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 1));
-      v[j][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 2));
-      v[j][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[j], f, 3));
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                      // column 8u + k: its four rows' values
-      const uint32_t pick = k & 1 ? 0x07060302u : 0x05040100u;
-      const Uint2 out = {__builtin_amdgcn_perm(v[1][k / 2], v[0][k / 2], pick), __builtin_amdgcn_perm(v[3][k / 2], v[2][k / 2], pick)};
-      *reinterpret_cast<Uint2*>(s_grad + (put_at ^ static_cast<uint32_t>(k * 64 + (k >> 2) * 16)) + buf * (kPanel * 64)) = out;
+    for (int k = 0; k < 4; ++k) {
+      Uint4 out;
+      out[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 0));
+      out[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 1));
+      out[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 2));
+      out[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 3));
+      *reinterpret_cast<Uint4*>(s_grad + (put_at ^ static_cast<uint32_t>(k << 4)) + buf * (kPanel * 64)) = out;
     }
   };
   Float16 acc[TI][TJ] = {};
-  const uint8_t* const read_w = s_grad + wk * 64;
   const uint8_t* const read_g = s_g + wm * 64;
-  const uint32_t place_w = static_cast<uint32_t>(short_row(turned(lane & 31), half)), place_g = static_cast<uint32_t>(short_row(lane & 31, half));
-  auto multiply = [&](int buf) {
+  const uint32_t place_g = static_cast<uint32_t>(short_row(lane & 31, half));
+  uint32_t place_w[TJ];                                // lane 16g + 4r + s: row r (+ 8 for the upper half of the wave), columns 16 (g % 2) + 4s ..
 #pragma unroll
-    for (int k = 0; k < kChunk / 16; ++k) {            // 16 of the contraction a matrix instruction: lane half h has chunk 2k + h
-      Bf16x8 b[TJ];
+  for (int j = 0; j < TJ; ++j)
+    place_w[j] = static_cast<uint32_t>(half * 4096 + wide_row(lane >> 2 & 3, (wk + j * 32) / 8 + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) + (lane & 1) * 8);
+  constexpr int K = kChunk / 16;                       // 16 of the contraction a matrix instruction: lane half h has eight, 16k + 8h ..
+  auto read = [&](int buf, Bf16x8 (&b)[K][TJ]) {
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) b[j] = *reinterpret_cast<const Bf16x8*>(read_w + (place_w ^ static_cast<uint32_t>(k * 32)) + buf * (kPanel * 64) + j * 2048);
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const uint8_t* p = s_grad + place_w[j] + buf * (kPanel * 64) + k * 8192;
+        b[k][j] = __builtin_shufflevector(read_turned(p), read_turned(p + 2048), 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+  };
+  auto multiply = [&](int buf, const Bf16x8 (&b)[K][TJ]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int s = 0; s < N; ++s) {
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
           const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(read_g + (place_g ^ static_cast<uint32_t>(k * 32)) + (buf * N + s) * kTermBytes + i * 2048);
 #pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[k][j], acc[i][j], 0, 0, 0);
         }
       }
     }
   };
 
-  Held h0, h1;
+  Held held[kHeld];                                    // chunk c is in held[c % kHeld]
   request(begin, 0);
-  __builtin_amdgcn_sched_barrier(0);                   // (the copies must be older than the eight loads that step() leaves on their way)
-  fetch(begin, h0);
-  fetch(min(begin + 1, last), h1);
-  turn(h0, 0);
-  fetch(min(begin + 2, last), h0);
-  // h: holds chunk c + 1, is given chunk c + 3
-  auto step = [&](int c, Held& h, int buf) {
+  __builtin_amdgcn_sched_barrier(0);                   // (the copies must be older than the two loads that step() leaves on their way)
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) fetch(min(begin + k, last), held[k]);
+  turn(held[0], 0);
+  fetch(min(begin + kHeld, last), held[0]);
+  auto step = [&](int c, Held& h, int buf) {           // h: holds chunk c + 1, is given chunk c + 1 + kHeld
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // chunk c's copies have landed: only the eight loads of chunk c + 2 came after
+    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // chunk c's copies have landed: only the two loads of chunk c + kHeld came after
+    Bf16x8 b[K][TJ];
+    read(buf, b);                                      // before the next copies are asked for: the compiler takes a turned read to depend on every copy on its way
+    __builtin_amdgcn_sched_barrier(0);
     request(min(c + 1, last), buf ^ 1);
     __builtin_amdgcn_sched_barrier(0);
     turn(h, buf ^ 1);
-    fetch(min(c + 3, last), h);
-    multiply(buf);
+    fetch(min(c + 1 + kHeld, last), h);
+    multiply(buf, b);
   };
-  for (int c = begin; c < end; c += 2) {               // (chunks come in pairs: the planes are padded to them)
-    step(c, h1, 0);
-    step(c + 1, h0, 1);
+  for (int c = begin; c < end; c += kHeld) {           // (chunks come in fours: the planes are padded to them)
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) step(c + k, held[(k + 1) % kHeld], k & 1);
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // no copy may land in an LDS that is another workgroup's by then
   float* to = partial + static_cast<int64_t>(part) * rows * cols;
@@ -678,11 +689,11 @@ struct GradPlan {
 };
 GradPlan plan_dgrad(int64_t m, int64_t n, int64_t k) {
   const int bm = m <= 32 ? 32 : (m <= 64 ? 64 : 128);
-  const int64_t pairs = (n + 2 * kChunk - 1) / (2 * kChunk), tiles = panels_of(k) * ((m + bm - 1) / bm);
+  const int64_t fours = (n + kHeld * kChunk - 1) / (kHeld * kChunk), tiles = panels_of(k) * ((m + bm - 1) / bm);
   int64_t s = (bm == 128 ? 512 : 768) / tiles;
-  if (s > pairs / 4) s = pairs / 4;
+  if (s > fours / 2) s = fours / 2;
   if (s < 1) s = 1;
-  return {bm, static_cast<int>(s), pairs * 2 * kChunk};
+  return {bm, static_cast<int>(s), fours * kHeld * kChunk};
 }
 int terms_of(int dtype) { return dtype == ADV_F32 ? 3 : (dtype == ADV_F16 ? 2 : 1); }
 int64_t plane_bytes(int64_t m, int64_t n, int dtype) { return padded(terms_of(dtype) * m * plan_dgrad(m, n, 1).padded_n * 2); }
