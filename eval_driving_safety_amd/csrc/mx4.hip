@@ -34,6 +34,30 @@ typedef uint32_t Uint4 __attribute__((ext_vector_type(4)));
 
 __host__ __device__ inline int64_t panels_of(int64_t cols) { return (cols + kPanel - 1) / kPanel; }
 
+struct Coded {
+  uint32_t code, scale;
+};
+// V consecutive values of a lane, 32 / V neighbouring lanes a block: their codes and the block's scale byte
+template <int V>
+__device__ __forceinline__ Coded encode(const float (&v)[V]) {
+  uint32_t top = 0;                        // the largest magnitude's bits: NaN and infinities come out on top
+#pragma unroll
+  for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < 32 / V; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+  const bool none = top >= 0x7f800000u;
+  const uint32_t scale = none ? 255u : static_cast<uint32_t>(max(static_cast<int>(top >> 23) - 2, 0));
+  const float unit = __uint_as_float(max(scale << 23, 0x00400000u));                 // 2^-127 is a subnormal
+  uint32_t q = 0;
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], unit, 0);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], unit, 1);
+  if (V == 8) {
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[V - 4], v[V - 3], unit, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[V - 2], v[V - 1], unit, 3);
+  }
+  return {none ? 0u : q, scale};
+}
+
 // ---- quantise / dequantise.  V elements (16 bytes) a lane, kPanel / V lanes a panel's row; a wave walks rows of one panel, so that what it
 //      writes is contiguous.  Bound by memory: 4.5 bytes moved a float32 value against ~6 instructions a lane's V values.
 constexpr int kRowsPerWave = 4;            // row groups a wave takes
@@ -55,27 +79,11 @@ __global__ __launch_bounds__(kBlock) void mx4_quantize(const T* __restrict__ x, 
     float v[V];
     if (left == V) lowp::load<T, V>(x + row * cols + col, v);
     else lowp::load_some<T, V>(x + row * cols + col, v, left);
-    uint32_t top = 0;                        // the largest magnitude's bits: NaN and infinities come out on top
-#pragma unroll
-    for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int d = 1; d < 32 / V; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
-    const bool none = top >= 0x7f800000u;
-    const int ex = static_cast<int>(top >> 23) - 2;
-    const uint32_t scale = none ? 255u : static_cast<uint32_t>(max(ex, 0));
-    const float unit = __uint_as_float(max(scale << 23, 0x00400000u));                 // 2^-127 is a subnormal
-    uint32_t q = 0;
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], unit, 0);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], unit, 1);
-    if (V == 8) {
-      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[V - 4], v[V - 3], unit, 2);
-      q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[V - 2], v[V - 1], unit, 3);
-    }
-    if (none) q = 0;
+    const Coded q = encode<V>(v);
     uint8_t* c = codes + (panel * rows + row) * (kPanel / 2) + in_row * (V / 2);
-    if (V == 8) *reinterpret_cast<uint32_t*>(c) = q;
-    else *reinterpret_cast<uint16_t*>(c) = static_cast<uint16_t>(q);
-    if (in_row % (32 / V) == 0) scales[(panel * rows + row) * 8 + in_row / (32 / V)] = static_cast<uint8_t>(scale);
+    if (V == 8) *reinterpret_cast<uint32_t*>(c) = q.code;
+    else *reinterpret_cast<uint16_t*>(c) = static_cast<uint16_t>(q.code);
+    if (in_row % (32 / V) == 0) scales[(panel * rows + row) * 8 + in_row / (32 / V)] = static_cast<uint8_t>(q.scale);
   }
 }
 
@@ -183,10 +191,16 @@ __device__ __forceinline__ void put_tile(__amdgpu_buffer_rsrc_t to, const Float1
 
 // Few rows of x: bound by reading W once.  16 rows of W (A) x 16 * MT rows of x (B) a workgroup on 16x16x128 instructions, operands straight
 // from memory to registers (a panel's 16 rows are 2 KB in one piece); the waves share the panels out and join their sums in LDS, in order.
-template <class T, int MT>
-__global__ __launch_bounds__(1024) void mx4_linear_thin(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y, int panels, int relu) {
-  extern __shared__ __attribute__((aligned(16))) float s_sum[];        // [wave][MT][4][64]
+// RAW: x comes as values (four rows at most); every workgroup quantises them for itself into LDS while its first piece of W is on its way - a second
+// reading of x from the L2 for every 16 rows of W, against a launch of its own (17.0 -> 13.6 us for one crop).
+template <class T, int MT, bool RAW>
+__global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __restrict__ values, int64_t cols, Operand w, const T* __restrict__ bias, T* __restrict__ y,
+                                                       int panels, int relu) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_thin[];     // sums [wave][MT][4][64]; RAW: codes [panel][row][128], scales [panel][row][8]
+  float* s_sum = reinterpret_cast<float*>(s_thin);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, quarter = lane >> 4;
+  uint8_t* s_codes = s_thin + waves * MT * 1024;
+  uint8_t* s_scales = s_codes + panels * static_cast<int>(RAW ? x.rows : 0) * 128;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, m0 = static_cast<int64_t>(blockIdx.y) * (16 * MT);
   const int64_t n = min(n0 + (lane & 15), w.rows - 1);                 // rows behind the last one are computed, not stored
   int64_t m[MT];
@@ -194,20 +208,56 @@ __global__ __launch_bounds__(1024) void mx4_linear_thin(Operand x, Operand w, co
 #pragma unroll
   for (int i = 0; i < MT; ++i) m[i] = min(m0 + 16 * i + (lane & 15), x.rows - 1);
   constexpr int U = MT == 1 ? 4 : 2;                                   // panels whose operands are on their way together
-  for (int p0 = wave; p0 < panels; p0 += waves * U) {
-    Uint4 a[U][2], b[U][MT][2];
-    uint32_t sa[U], sb[U][MT];
+  Uint4 a[U][2];
+  uint32_t sa[U];
+  auto fetch = [&](int p0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t p = min(p0 + u * waves, panels - 1);
       const Uint4* at = reinterpret_cast<const Uint4*>(w.codes + (p * w.rows + n) * 128 + quarter * 32);
       a[u][0] = at[0], a[u][1] = at[1];
       sa[u] = *reinterpret_cast<const uint16_t*>(w.scales + (p * w.rows + n) * 8 + quarter * 2);
+    }
+  };
+  fetch(wave);
+  if constexpr (RAW) {
+    constexpr int V = 16 / sizeof(T), kLanes = kPanel / V, kGroup = 64 / kLanes;      // lanes a panel's row, rows a wave takes at once
+    constexpr int kBatch = V == 4 ? 7 : 4;                             // pieces whose values are on their way together
+    const int pieces = panels * static_cast<int>(x.rows), rows = static_cast<int>(x.rows), in_row = lane % kLanes, step = waves * kGroup;
+    for (int i0 = wave * kGroup + lane / kLanes; i0 < pieces; i0 += kBatch * step) {
+      float v[kBatch][V];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = min(i0 + k * step, pieces - 1), p = i / rows, row = i - p * rows;
+        const int64_t col = static_cast<int64_t>(p) * kPanel + in_row * V;
+        const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(V), cols - col)));
+        if (left == V) lowp::load<T, V, false>(values + row * cols + col, v[k]);
+        else lowp::load_some<T, V>(values + row * cols + col, v[k], left);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * step;
+        if (i >= pieces) break;                                        // (whole rows of lanes leave together)
+        const Coded q = encode<V>(v[k]);
+        if (V == 8) *reinterpret_cast<uint32_t*>(s_codes + i * 128 + in_row * 4) = q.code;
+        else *reinterpret_cast<uint16_t*>(s_codes + i * 128 + in_row * 2) = static_cast<uint16_t>(q.code);
+        if (in_row % (32 / V) == 0) s_scales[i * 8 + in_row / (32 / V)] = static_cast<uint8_t>(q.scale);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");    // (__syncthreads would also wait for W)
+  }
+  for (int p0 = wave; p0 < panels;) {
+    Uint4 b[U][MT][2];
+    uint32_t sb[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t p = min(p0 + u * waves, panels - 1);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const Uint4* bt = reinterpret_cast<const Uint4*>(x.codes + (p * x.rows + m[i]) * 128 + quarter * 32);
+        const int64_t row = p * x.rows + m[i];
+        const Uint4* bt = reinterpret_cast<const Uint4*>((RAW ? s_codes : x.codes) + row * 128 + quarter * 32);
         b[u][i][0] = bt[0], b[u][i][1] = bt[1];
-        sb[u][i] = *reinterpret_cast<const uint16_t*>(x.scales + (p * x.rows + m[i]) * 8 + quarter * 2);
+        sb[u][i] = *reinterpret_cast<const uint16_t*>((RAW ? s_scales : x.scales) + row * 8 + quarter * 2);
       }
     }
 #pragma unroll
@@ -222,6 +272,8 @@ __global__ __launch_bounds__(1024) void mx4_linear_thin(Operand x, Operand w, co
         }
       }
     }
+    p0 += waves * U;
+    if (p0 < panels) fetch(p0);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -385,10 +437,10 @@ __global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ par
   if (left <= 0) return;
   float v[4];
   if (left == 4) {
-    lowp::load<float, 4>(partial + i, v);
+    lowp::load<float, 4, false>(partial + i, v);
     for (int k = 1; k < parts; ++k) {
       float p[4];
-      lowp::load<float, 4>(partial + k * n + i, p);
+      lowp::load<float, 4, false>(partial + k * n + i, p);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += p[j];
     }
@@ -651,21 +703,31 @@ int run_dequantize(const uint8_t* codes, const uint8_t* scales, void* x, int64_t
 constexpr int64_t kAlign = 256;
 int64_t padded(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
 
-// How a product is cut: thin tiles up to 64 rows; above, 256 x 256 tiles where they fill half the chip, else 128 x 128, the panels dealt to
-// several workgroups a tile where tiles alone do not fill it (at least four panels each: a workgroup's start and the joining pass cost about two).
+// How a product is cut.
+//   thin   up to 16 rows, and up to 64 against a weight of 2^23 values or fewer: one launch (4096 x 1000: 16 against 19 us at 64 rows); with
+//          25088 x 4096 tiles are faster from 17 rows on (64 rows: 22 against 39 us), as every 16 rows of W read all of x again there.
+//   big    256 x 256 tiles where there are 128 of them or more, else 128 x 128.
+//   splits the panels are dealt to several workgroups a tile where tiles alone do not fill the chip: the number with the least estimated time, from
+//          0.8 us a panel with one 128 x 128 workgroup a CU, 1.1 us with two (measured at 32 .. 256 rows of 25088 x 4096), three panels' time for a
+//          workgroup's start and end, and the joining pass at 8 TB/s (the parts are in the caches).
 struct LinearPlan {
   int thin, big, splits;
 };
 LinearPlan plan_linear(int64_t m, int64_t n, int64_t k) {
   const int64_t panels = panels_of(k);
-  if (m <= 64) return {1, 0, 1};
+  if (m <= 16 || (m <= 64 && n * k <= (int64_t{1} << 23))) return {1, 0, 1};
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-  const bool use_big = big >= 128;
-  const int64_t tiles = use_big ? big : small, room = use_big ? 256 : 512;
-  int64_t s = room / tiles;
-  if (s > panels / 4) s = panels / 4;
-  if (s < 1) s = 1;
-  return {0, use_big ? 1 : 0, static_cast<int>(s)};
+  if (big >= 128) return {0, 1, static_cast<int>(big >= 256 || panels < 8 ? 1 : 256 / big)};
+  int best = 1;
+  double least = 0.0;
+  for (int64_t s = 1; s <= 32 && (s == 1 || s <= panels / 4); ++s) {
+    const int64_t groups = small * s;
+    const double each = static_cast<double>((panels + s - 1) / s + 3);
+    double t = groups <= 256 ? 0.8 * each : 1.1 * each * static_cast<double>((groups + 511) / 512);
+    if (s > 1) t += 2.0 + 1e-6 * static_cast<double>(s * m * n);
+    if (s == 1 || t < least) best = static_cast<int>(s), least = t;
+  }
+  return {0, 0, best};
 }
 int64_t linear_partial_bytes(int64_t m, int64_t n, int64_t k) {
   const LinearPlan p = plan_linear(m, n, k);
@@ -679,12 +741,17 @@ void run_join(const float* partial, const void* bias, void* y, int64_t rows, int
                                                                                          relu);
 }
 
-template <class T, int MT>
-int run_thin(Operand x, Operand w, const void* bias, void* y, int panels, int relu, hipStream_t st) {
-  const int waves = panels >= 16 ? 16 : (panels >= 4 ? 4 : 1), lds = waves * MT * 1024;
+constexpr int kThinLds = 64 * 1024;        // a workgroup's share: two on a CU
+int thin_waves(int panels) { return panels >= 16 ? 8 : (panels >= 4 ? 4 : 1); }
+// the rows of x fit a thin workgroup's LDS in four bits
+bool thin_raw(int64_t m, int64_t k) { return m <= 4 && panels_of(k) * m * 136 + 8 * 1024 <= kThinLds; }
+
+template <class T, int MT, bool RAW>
+int run_thin(Operand x, const void* values, int64_t k, Operand w, const void* bias, void* y, int relu, hipStream_t st) {
+  const int panels = static_cast<int>(panels_of(k)), waves = thin_waves(panels);
+  const int lds = waves * MT * 1024 + (RAW ? panels * static_cast<int>(x.rows) * 136 : 0);
   const dim3 grid(static_cast<unsigned>((w.rows + 15) / 16), static_cast<unsigned>((x.rows + 16 * MT - 1) / (16 * MT)));
-  if (!adv_internal_lds_limit<mx4_linear_thin<T, MT>>(16 * MT * 1024)) return ADV_ELAUNCH;
-  mx4_linear_thin<T, MT><<<grid, waves * 64, lds, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), panels, relu);
+  mx4_linear_thin<T, MT, RAW><<<grid, waves * 64, lds, st>>>(x, static_cast<const T*>(values), k, w, static_cast<const T*>(bias), static_cast<T*>(y), panels, relu);
   return adv_internal_finish_launch();
 }
 
@@ -698,15 +765,24 @@ int run_tile(Operand x, Operand w, const void* bias, void* y, float* partial, in
   return adv_internal_finish_launch();
 }
 
+// x: codes and scales, or - x.codes NULL - ``values``, which are quantised into ``ws``
 template <class T>
-int run_linear(Operand x, Operand w, const void* bias, void* y, float* partial, int64_t k, int relu, hipStream_t st) {
+int run_linear(Operand x, const void* values, Operand w, const void* bias, void* y, uint8_t* ws, int64_t k, int relu, hipStream_t st) {
   const LinearPlan p = plan_linear(x.rows, w.rows, k);
-  const int panels = static_cast<int>(panels_of(k));
-  if (p.thin) {
-    if (x.rows <= 16) return run_thin<T, 1>(x, w, bias, y, panels, relu, st);
-    if (x.rows <= 32) return run_thin<T, 2>(x, w, bias, y, panels, relu, st);
-    return run_thin<T, 4>(x, w, bias, y, panels, relu, st);
+  if (!x.codes && p.thin && thin_raw(x.rows, k)) return run_thin<T, 1, true>(x, values, k, w, bias, y, relu, st);
+  const int64_t cb = padded(code_bytes(x.rows, k)), sb = padded(scale_bytes(x.rows, k));
+  if (!x.codes) {
+    const int bad = run_quantize<T>(values, ws, ws + cb, x.rows, k, st);
+    if (bad) return bad;
+    x.codes = ws, x.scales = ws + cb;
   }
+  if (p.thin) {
+    if (x.rows <= 16) return run_thin<T, 1, false>(x, nullptr, k, w, bias, y, relu, st);
+    if (x.rows <= 32) return run_thin<T, 2, false>(x, nullptr, k, w, bias, y, relu, st);
+    return run_thin<T, 4, false>(x, nullptr, k, w, bias, y, relu, st);
+  }
+  float* partial = reinterpret_cast<float*>(ws + cb + sb);
+  const int panels = static_cast<int>(panels_of(k));
   if (p.big) return run_tile<T, 256, 256>(x, w, bias, y, partial, panels, p.splits, relu, st);
   return run_tile<T, 128, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
 }
@@ -803,18 +879,10 @@ int adv_mx4_linear(const void* x, const uint8_t* x_codes, const uint8_t* x_scale
     if (b.at && (lowp::overlap(y, yb, b.at, b.bytes) || lowp::overlap(workspace, wb, b.at, b.bytes))) return ADV_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (x) {
-    uint8_t* scales = ws + padded(code_bytes(m, k));
-    const int bad = dtype == ADV_F32 ? run_quantize<float>(x, ws, scales, m, k, st)
-                                     : (dtype == ADV_BF16 ? run_quantize<__bf16>(x, ws, scales, m, k, st) : run_quantize<_Float16>(x, ws, scales, m, k, st));
-    if (bad) return bad;
-    x_codes = ws, x_scales = scales;
-  }
-  float* partial = reinterpret_cast<float*>(ws + padded(code_bytes(m, k)) + padded(scale_bytes(m, k)));
   const Operand xo{x_codes, x_scales, m}, wo{w_codes, w_scales, n};
-  if (dtype == ADV_F32) return run_linear<float>(xo, wo, bias, y, partial, k, relu, st);
-  if (dtype == ADV_BF16) return run_linear<__bf16>(xo, wo, bias, y, partial, k, relu, st);
-  return run_linear<_Float16>(xo, wo, bias, y, partial, k, relu, st);
+  if (dtype == ADV_F32) return run_linear<float>(xo, x, wo, bias, y, ws, k, relu, st);
+  if (dtype == ADV_BF16) return run_linear<__bf16>(xo, x, wo, bias, y, ws, k, relu, st);
+  return run_linear<_Float16>(xo, x, wo, bias, y, ws, k, relu, st);
 }
 
 int64_t adv_mx4_linear_dgrad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype) {

@@ -31,4 +31,4 @@ from .boxes import *       # noqa: F401,F403
 from .dropout import *       # noqa: F401,F403
 from .mx4 import *       # noqa: F401,F403
 
-SOURCES = tuple(__import__("os").path.join(__import__("os").path.dirname(__file__), n + ".py") for n in ("_base", "elementwise", "pixel", "psv", "roi", "conv3d", "conv2d", "wino4", "align", "volume", "boxes", "dropout", "mx4"))
+SOURCES = tuple(__import__("os").path.join(__import__("os").path.dirname(__file__), n + ".py") for n in ("_base", "_lowp", "elementwise", "pixel", "psv", "roi", "conv3d", "conv2d", "wino4", "align", "volume", "boxes", "dropout", "mx4"))

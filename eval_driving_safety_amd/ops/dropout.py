@@ -1,26 +1,6 @@
 """dropout of a fully connected head, its mask from a counter-based generator and never stored (csrc/dropout.hip).  Part of the ``ops``
 package."""
-from ._base import *       # noqa: F401,F403  (torch, ctypes, _lib and the argument helpers)
-
-_FLOATS = {torch.float32: _lib.ADV_F32, torch.bfloat16: _lib.ADV_BF16, torch.float16: _lib.ADV_F16}
-
-
-def _head(t, name, like=None):
-    """a contiguous float32 / bfloat16 / float16 ROCm tensor (of ``like``'s type and device)"""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _FLOATS and t.is_contiguous()):
-        raise TypeError("%s must be a contiguous float32, bfloat16 or float16 CUDA tensor" % name)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError("%s (%s on %s) must have the type and device of the tensor it belongs to (%s on %s)" % (name, t.dtype, t.device, like.dtype, like.device))
-    return t
-
-
-def _matrix(t):
-    """(rows, columns) of a tensor whose last dimension is the layer's"""
-    if t.dim() < 1:
-        raise ValueError("a tensor of at least one dimension is needed")
-    cols = t.shape[-1]
-    return (t.numel() // cols if cols else 0), cols
-
+from ._lowp import *       # noqa: F401,F403  (torch, _lib and the argument helpers)
 
 def _draw(p, seed, step, like):
     """the generator's arguments of the C calls, checked: (p, seed, step_at, step)"""
@@ -54,10 +34,9 @@ def dropout(x, p, seed, step=0, bias=None, relu=False, out=None):
         out = torch.empty_like(x)
     elif _head(out, "out", x).shape != x.shape:
         raise ValueError("out must have x's shape")
-    if x.numel():
-        with _on(x):
-            _lib.call("adv_dropout_fwd", x.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), rows, cols, _FLOATS[x.dtype],
-                      p, seed, step_at, step, 1 if relu else 0, _stream(x))
+    if rows and cols:
+        _enqueue("adv_dropout_fwd", x.device, x.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), rows, cols, _FLOATS[x.dtype],
+                 p, seed, step_at, step, 1 if relu else 0)
     return out
 
 
@@ -74,16 +53,16 @@ def dropout_bwd(grad_y, p, seed, step=0, y=None, with_bias=False, out=None):
         out = torch.empty_like(grad_y)
     elif _head(out, "out", grad_y).shape != grad_y.shape:
         raise ValueError("out must have grad_y's shape")
-    if not grad_y.numel():
-        return out, torch.zeros((cols,), dtype=grad_y.dtype, device=grad_y.device) if with_bias else None
+    if not (rows and cols):
+        return out, grad_y.new_zeros((cols,)) if with_bias else None
     gbias = ws = None
-    with _on(grad_y):
-        if with_bias:
-            gbias = torch.empty((cols,), dtype=grad_y.dtype, device=grad_y.device)
-            n = _lib.load().adv_dropout_bwd_workspace_floats(rows, cols, _FLOATS[grad_y.dtype])
-            ws = torch.empty((n,), dtype=torch.float32, device=grad_y.device) if n > 0 else None
-        _lib.call("adv_dropout_bwd", grad_y.data_ptr(), None if y is None else y.data_ptr(), out.data_ptr(), None if gbias is None else gbias.data_ptr(),
-                  None if ws is None else ws.data_ptr(), rows, cols, _FLOATS[grad_y.dtype], p, seed, step_at, step, _stream(grad_y))
+    kind = _FLOATS[grad_y.dtype]
+    if with_bias:
+        gbias = grad_y.new_empty((cols,))
+        n = _workspace("adv_dropout_bwd_workspace_floats", rows, cols, kind)
+        ws = grad_y.new_empty((n,), dtype=torch.float32) if n else None
+    _enqueue("adv_dropout_bwd", grad_y.device, grad_y.data_ptr(), None if y is None else y.data_ptr(), out.data_ptr(), None if gbias is None else gbias.data_ptr(),
+             None if ws is None else ws.data_ptr(), rows, cols, kind, p, seed, step_at, step)
     return out, gbias
 
 

@@ -1,7 +1,6 @@
 """matrices held in MXFP4 (32 values of a row as 4-bit floats under one power of two) and their products on the scaled matrix instructions
 (csrc/mx4.hip): a fully connected head with four-bit weights, served or attacked.  Part of the ``ops`` package."""
-from ._base import *       # noqa: F401,F403  (torch, ctypes, _lib and the argument helpers)
-from .dropout import _FLOATS, _head, _matrix
+from ._lowp import *       # noqa: F401,F403  (torch, _lib and the argument helpers)
 
 _PANEL = 256               # columns of a panel of the layout: 128 code bytes and 8 scale bytes a row
 
@@ -53,11 +52,9 @@ def mx4_quantize(x):
     if cols < 1:
         raise ValueError("x needs at least one column")
     panels = (cols + _PANEL - 1) // _PANEL
-    codes = torch.empty((panels, rows, 128), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((panels, rows, 8), dtype=torch.uint8, device=x.device)
+    codes, scales = x.new_empty((panels, rows, 128), dtype=torch.uint8), x.new_empty((panels, rows, 8), dtype=torch.uint8)
     if rows:
-        with _on(x):
-            _lib.call("adv_mx4_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols, _FLOATS[x.dtype], _stream(x))
+        _enqueue("adv_mx4_quantize", x.device, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, cols, _FLOATS[x.dtype])
     return Mx4(codes, scales, x.shape)
 
 
@@ -66,10 +63,9 @@ def mx4_dequantize(q, dtype=torch.float32):
     _mx4(q, "q")
     if dtype not in _FLOATS:
         raise TypeError("dtype must be float32, bfloat16 or float16")
-    x = torch.empty(q.shape, dtype=dtype, device=q.device)
+    x = q.codes.new_empty(q.shape, dtype=dtype)
     if q.rows:
-        with _on(x):
-            _lib.call("adv_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), x.data_ptr(), q.rows, q.cols, _FLOATS[dtype], _stream(x))
+        _enqueue("adv_mx4_dequantize", q.device, q.codes.data_ptr(), q.scales.data_ptr(), x.data_ptr(), q.rows, q.cols, _FLOATS[dtype])
     return x
 
 
@@ -98,18 +94,17 @@ def mx4_linear(x, w, bias=None, relu=False, dtype=None):
     if len(x.shape) < 1 or x.shape[-1] != w.cols:
         raise ValueError("x %s does not fit a weight of %d columns" % (tuple(x.shape), w.cols))
     _same_device(w, x, bias)
-    y = torch.empty(tuple(x.shape[:-1]) + (w.rows,), dtype=dtype, device=w.device)
+    y = w.codes.new_empty(x.shape[:-1] + (w.rows,), dtype=dtype)
     if bias is not None and tuple(_head(bias, "bias", y).shape) != (w.rows,):
         raise ValueError("bias must be [%d], got %s" % (w.rows, tuple(bias.shape)))
-    if not y.numel():
-        return y
+    m, n, k = x.shape[:-1].numel(), w.rows, w.cols
     held = _mx4(x, "x") if isinstance(x, Mx4) else None
-    m = y.numel() // w.rows
-    with _on(y):
-        ws = torch.empty((_lib.load().adv_mx4_linear_workspace_bytes(m, w.rows, w.cols),), dtype=torch.uint8, device=y.device)
-        _lib.call("adv_mx4_linear", x.data_ptr() if held is None else None, None if held is None else held.codes.data_ptr(),
-                  None if held is None else held.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                  y.data_ptr(), ws.data_ptr(), m, w.rows, w.cols, _FLOATS[dtype], 1 if relu else 0, _stream(y))
+    if not (m and n):
+        return y
+    ws = y.new_empty((_workspace("adv_mx4_linear_workspace_bytes", m, n, k),), dtype=torch.uint8)
+    _enqueue("adv_mx4_linear", y.device, x.data_ptr() if held is None else None, None if held is None else held.codes.data_ptr(),
+             None if held is None else held.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+             y.data_ptr(), ws.data_ptr(), m, n, k, _FLOATS[dtype], 1 if relu else 0)
     return y
 
 
@@ -124,16 +119,15 @@ def mx4_linear_dgrad(grad_y, w, mask=None):
     if mask is not None and _head(mask, "mask", grad_y).shape != grad_y.shape:
         raise ValueError("mask must have grad_y's shape")
     _same_device(w, grad_y)
-    gx = torch.empty(tuple(grad_y.shape[:-1]) + (w.cols,), dtype=grad_y.dtype, device=w.device)
-    if not gx.numel():
+    gx = grad_y.new_empty(grad_y.shape[:-1] + (w.cols,))
+    m, n, k, kind = grad_y.shape[:-1].numel(), w.rows, w.cols, _FLOATS[gx.dtype]
+    if not m:
         return gx
-    if not w.rows:
+    if not n:
         return gx.zero_()
-    m, kind = gx.numel() // w.cols, _FLOATS[gx.dtype]
-    with _on(gx):
-        ws = torch.empty((_lib.load().adv_mx4_linear_dgrad_workspace_bytes(m, w.rows, w.cols, kind),), dtype=torch.uint8, device=gx.device)
-        _lib.call("adv_mx4_linear_dgrad", grad_y.data_ptr(), None if mask is None else mask.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), gx.data_ptr(),
-                  ws.data_ptr(), m, w.rows, w.cols, kind, _stream(gx))
+    ws = gx.new_empty((_workspace("adv_mx4_linear_dgrad_workspace_bytes", m, n, k, kind),), dtype=torch.uint8)
+    _enqueue("adv_mx4_linear_dgrad", gx.device, grad_y.data_ptr(), None if mask is None else mask.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+             gx.data_ptr(), ws.data_ptr(), m, n, k, kind)
     return gx
 
 
