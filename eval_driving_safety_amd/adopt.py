@@ -13,6 +13,8 @@ The attacks differentiate w.r.t. the images only; the detector is in eval mode a
   * a stride-2 1x1 layer (ResNet's down-sampling projections) is a sub-sampling copy + the 1x1 GEMM kernel;
   * layers without a kernel here (7x7 stems, strided 3x3 layers, grouped convolutions ...) keep torch's operator but still lose their
     BatchNorm (folded) and get bias + ReLU as ONE fused pass (``ops.bias_act_``);
+  * on request (``linear="mxfp4"``) every ``nn.Linear`` is evaluated and attacked as deployed in four bits: weights held in MXFP4, inputs quantised on
+    the way in, the gradient straight through (``heads.Mx4LinearLayer`` on csrc/mx4.hip);
   * gradients flow to the INPUT only: the adopted modules return no weight gradients (``adopt`` switches ``requires_grad`` off on
     what it adopts, as adapters._freeze does for the whole model).
 
@@ -245,15 +247,18 @@ def _make(conv, bn, relu):
     return _CONVS[type(conv)](conv, w, b, relu)
 
 
-def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, freeze=True, functional=True):
+def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, freeze=True, functional=True, linear=None):
     """Replace, IN PLACE, the convolutions of ``model`` by libadvengine-backed modules carrying the model's own weights (see the module
     docstring).  ``functional``: also bind the two functional patterns of a DSGN forward - 5-D ``F.grid_sample`` and the
     ``F.interpolate(trilinear)`` -> softmax -> depth-weighted sum chain - to ``ops.GridSample3d`` / ``ops.DepthRegress`` by putting a proxy
     where the defining Python modules hold ``torch.nn.functional`` (adopt_functional.py; ``adopt_functional.unbind()`` undoes it).
+    ``linear="mxfp4"``: the model's ``nn.Linear`` layers with four-bit weights - another model, a few per cent off: give ``verify`` a ``tol`` to match.
     -> {"replaced": [(qualified name, what)], "folded_bn": n, "fused_relu": n, "kept": [(name, why)], "upsample_add": modules whose
     ``_upsample_add`` now has a deterministic backward, "functional": [(python module, global name)] rebound}."""
     if model.training:
         raise ValueError("adopt() needs the model in eval mode (BatchNorm statistics are folded)")
+    if linear not in (None, "mxfp4"):
+        raise ValueError("linear must be None or 'mxfp4', got %r" % (linear,))
     before = rng = None
     if verify is not None:
         rng = _rng_snapshot()
@@ -303,6 +308,9 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
                 setattr(parent, bn_name, nn.Identity())
                 report["folded_bn"] += 1
             report["replaced"].append((_q(parent_name, name), getattr(parent, name).kind))
+    if linear is not None:
+        from . import heads
+        report["replaced"] += heads.mx4_linears(model)
     for name, m in model.named_modules():
         if isinstance(m, (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.ConvTranspose2d, nn.ConvTranspose3d)):
             report["kept"].append((name, type(m).__name__ + ": no libadvengine counterpart for this module type here"))

@@ -5,7 +5,8 @@
 
 They are NOT on the perturbation hot path (standard fine-tunes whose only link to the attacks is through files: the
 evaluation scripts read their decisions as the presence of a label file, evaluation/convert_scenarios.py:40-42,109-112),
-so this is plain torch running on MIOpen - no custom kernels.  What is reproduced: the architectures with torchvision's
+so this is plain torch running on MIOpen; on request the heads take this package's kernels: a dropout whose masks are the same in every process
+(``train(dropout_seed=)``) and four-bit weights (``quantize_head``).  What is reproduced: the architectures with torchvision's
 parameter names (torchvision is absent here; the reference's checkpoints ``cnn_N.pth`` and torchvision's ImageNet
 weights load by key), the heads, the frozen-backbone rule, the transforms, the optimiser / learning-rate rules, the
 accuracy count and the checkpoint format.
@@ -155,6 +156,14 @@ def freeze_backbone(model, train_backbone=False):
         p.requires_grad = True if model.head_key in name else train_backbone
 
 
+def quantize_head(model):
+    """the head's Linear layers with their weights in MXFP4 (``heads.Mx4LinearLayer``), in place, for ``check_accuracy`` and for gradients w.r.t. the
+    images; the backbone stays as it is.  Needs a ROCm device when it runs.  -> [(qualified name, what)]"""
+    from . import heads
+    head = getattr(model.backbone, model.head_key)
+    return heads.mx4_linears(head, prefix=model.head_key + ".")
+
+
 # ------------------------------------------------------------------------------------------------ data
 def to_tensor_224(img, mean, std, flip=False):
     """transforms.Resize((224, 224)) [PIL bilinear] -> (RandomHorizontalFlip) -> ToTensor -> Normalize"""
@@ -215,15 +224,21 @@ TASKS = {
 }
 
 
-def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=None, train_backbone=False, log=print):
+def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=None, train_backbone=False, log=print, dropout_seed=None):
     """the training loops of dynamic_vehicles/train.py:87-125 and driving_constraint/train.py:91-118.
 
     dynamic_vehicles halves the learning rate once from epoch 6 and once from epoch 10 (:104-114).  driving_constraint
     builds a MultiStepLR([5, 10, 15], 0.1) but never steps it (:66-67 and no ``scheduler.step()`` anywhere), so its
-    learning rate stays 1e-3 - kept."""
+    learning rate stays 1e-3 - kept.
+
+    ``dropout_seed``: the head's Linear - Dropout - ReLU runs on ``ops.Dropout`` under this seed - the masks are a function of the seed and the step,
+    not of the process's generator (None: torch's dropout, as the scripts have it)."""
     cls, lr, n_epochs, _, val_every, save_every, _ = TASKS[task]
     model = (cls() if model is None else model).to(device)
     freeze_backbone(model, train_backbone)
+    if dropout_seed is not None:
+        from . import heads
+        heads.counter_dropout(getattr(model.backbone, model.head_key), dropout_seed)
     criterion = nn.BCELoss()
     optimizer = torch.optim.Adam(model.parameters(), lr=lr)
     os.makedirs(save_dir, exist_ok=True)

@@ -21,6 +21,8 @@ def build_parser():
     p.add_argument("--imagenet_weights", default=None, help="torchvision state dict of the backbone (pretrained=True of Model.py:19; no network here)")
     p.add_argument("--epochs", type=int, default=None, help="passes over the split")
     p.add_argument("--device", default=None)
+    p.add_argument("--dropout_seed", type=int, default=None, help="train: the head's dropout masks are drawn by a counter-based generator under this seed (the same in every run; needs a ROCm device)")
+    p.add_argument("--head", choices=["float32", "mxfp4"], default="float32", help="validate: the head's weights as they are, or held in four bits (needs a ROCm device)")
     return p
 
 
@@ -38,6 +40,9 @@ def main(argv=None):
     model = cls()
     if args.mode == "validate":
         C.load_checkpoint(model, args.checkpoint or "model/pretrained_model/cnn_20.pth")
+        if args.head == "mxfp4":
+            for name, what in C.quantize_head(model):
+                print("%s: %s" % (name, what))
         C.check_accuracy(val, model.to(dev), dev)
         return
     if args.imagenet_weights:
@@ -45,7 +50,7 @@ def main(argv=None):
     else:
         print("warning: no --imagenet_weights: the backbone starts from random weights (the reference starts from ImageNet)")
     train = torch.utils.data.DataLoader(C.CsvImageDataset(img, tcsv, cls.mean, cls.std, random_flip=flip), batch_size=batch, **kw)
-    C.train(args.task, train, val, dev, args.save_dir, epochs=args.epochs, model=model)
+    C.train(args.task, train, val, dev, args.save_dir, epochs=args.epochs, model=model, dropout_seed=args.dropout_seed)
 
 
 if __name__ == "__main__":

@@ -72,14 +72,18 @@ __global__ __launch_bounds__(kBlock) void mx4_quantize(const T* __restrict__ x, 
   const int64_t col = panel * kPanel + in_row * V;
   const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(V), cols - col)));
   const int64_t row0 = ((static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + wave) * kRowsPerWave) * kGroup + lane / kLanes;
+  float v[kRowsPerWave][V];                  // every row's values are asked for before the first is used
+#pragma unroll
+  for (int k = 0; k < kRowsPerWave; ++k) {
+    const int64_t row = min(row0 + k * kGroup, rows - 1);
+    if (left == V) lowp::load<T, V>(x + row * cols + col, v[k]);
+    else lowp::load_some<T, V>(x + row * cols + col, v[k], left);
+  }
 #pragma unroll
   for (int k = 0; k < kRowsPerWave; ++k) {
     const int64_t row = row0 + k * kGroup;
-    if (row >= rows) continue;               // (whole rows of lanes leave together: the exchanges below stay within one)
-    float v[V];
-    if (left == V) lowp::load<T, V>(x + row * cols + col, v);
-    else lowp::load_some<T, V>(x + row * cols + col, v, left);
-    const Coded q = encode<V>(v);
+    if (row >= rows) break;                  // (whole rows of lanes leave together: the exchanges in encode() stay within one)
+    const Coded q = encode<V>(v[k]);
     uint8_t* c = codes + (panel * rows + row) * (kPanel / 2) + in_row * (V / 2);
     if (V == 8) *reinterpret_cast<uint32_t*>(c) = q.code;
     else *reinterpret_cast<uint16_t*>(c) = static_cast<uint16_t>(q.code);
@@ -98,22 +102,28 @@ __global__ __launch_bounds__(kBlock) void mx4_dequantize(const uint8_t* __restri
   const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(V), cols - col)));
   if (left == 0) return;
   const int64_t row0 = ((static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + wave) * kRowsPerWave) * kGroup + lane / kLanes;
+  uint32_t q[kRowsPerWave], scale[kRowsPerWave];
+#pragma unroll
+  for (int k = 0; k < kRowsPerWave; ++k) {
+    const int64_t at = panel * rows + min(row0 + k * kGroup, rows - 1);
+    const uint8_t* c = codes + at * (kPanel / 2) + in_row * (V / 2);
+    q[k] = V == 8 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+    scale[k] = scales[at * 8 + in_row / (32 / V)];
+  }
 #pragma unroll
   for (int k = 0; k < kRowsPerWave; ++k) {
     const int64_t row = row0 + k * kGroup;
-    if (row >= rows) continue;
-    const uint8_t* c = codes + (panel * rows + row) * (kPanel / 2) + in_row * (V / 2);
-    const uint32_t q = V == 8 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-    const float unit = __uint_as_float(static_cast<uint32_t>(scales[(panel * rows + row) * 8 + in_row / (32 / V)]) << 23);
+    if (row >= rows) break;
+    const float unit = __uint_as_float(scale[k] << 23);
     float v[V];
-    Float2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, unit, 0);
+    Float2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[k], unit, 0);
     v[0] = p.x, v[1] = p.y;
-    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, unit, 1);
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[k], unit, 1);
     v[2] = p.x, v[3] = p.y;
     if (V == 8) {
-      p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, unit, 2);
+      p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[k], unit, 2);
       v[V - 4] = p.x, v[V - 3] = p.y;
-      p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, unit, 3);
+      p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[k], unit, 3);
       v[V - 2] = p.x, v[V - 1] = p.y;
     }
     if (left == V) lowp::store<T, V>(x + row * cols + col, v);

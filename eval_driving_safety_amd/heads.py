@@ -1,0 +1,113 @@
+"""Fully connected layers on libadvengine's kernels: trained with a counter-based dropout, or served / attacked with four-bit weights.
+
+``LinearDropout`` stands for Linear - Dropout (- ReLU) of a head in training (dynamic_vehicles/Model.py:24-27, driving_constraint/Model.py:21-23):
+the product is torch's, bias + dropout + ReLU are one kernel (``ops.Dropout``), and the mask of step s under a seed is the same in every process.
+``Mx4LinearLayer`` stands for a frozen Linear (- ReLU) whose weight is held in MXFP4 (``ops.Mx4Linear``): gradients flow to its input only, as
+through every adopted layer."""
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+
+def layer_seed(seed, index):
+    """another key for every dropout layer of a model"""
+    return (int(seed) + index * 0x9E3779B97F4A7C15) % (1 << 64)
+
+
+class LinearDropout(nn.Linear):
+    """``relu?(dropout(linear(x)))`` with ``nn.Linear``'s parameters and state-dict keys.  In training every forward takes the next ``step`` (a plain
+    number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device."""
+
+    def __init__(self, linear, p, seed, relu=False):
+        nn.Module.__init__(self)
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        self.weight, self.bias = linear.weight, linear.bias
+        self.p, self.seed, self.relu, self.step = float(p), int(seed), bool(relu), 0
+
+    def forward(self, x):
+        if not self.training:
+            y = F.linear(x, self.weight, self.bias)
+            return F.relu(y) if self.relu else y
+        from . import ops
+        step, self.step = self.step, self.step + 1
+        return ops.Dropout.apply(F.linear(x, self.weight), self.p, self.seed, step, self.bias, self.relu)
+
+    def extra_repr(self):
+        return "%s, p=%g, seed=%d, relu=%s" % (nn.Linear.extra_repr(self), self.p, self.seed, self.relu)
+
+
+class Mx4LinearLayer(nn.Module):
+    """``relu?(linear(x))`` with the weight in MXFP4 and x quantised on the way in; the weight is quantised when the layer first runs on a ROCm device
+    (its float32 copy is given up then)"""
+
+    def __init__(self, linear, relu=False):
+        super().__init__()
+        self.in_features, self.out_features, self.relu = linear.in_features, linear.out_features, bool(relu)
+        self.register_buffer("weight", linear.weight.detach().clone())
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+        self.register_buffer("codes", None)
+        self.register_buffer("scales", None)
+
+    def held(self):
+        """the weight as ``ops.Mx4``"""
+        from . import ops
+        if self.codes is None:
+            if not self.weight.is_cuda:
+                raise RuntimeError("Mx4LinearLayer: libadvengine has no CPU path - move the model and its inputs to the ROCm device")
+            q = ops.mx4_quantize(self.weight.contiguous())
+            self.codes, self.scales, self.weight = q.codes, q.scales, None
+        return ops.Mx4(self.codes, self.scales, (self.out_features, self.in_features))
+
+    def forward(self, x):
+        w = self.held()
+        from . import ops
+        bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
+        return ops.Mx4Linear.apply(x.contiguous(), w, bias, self.relu)
+
+    def extra_repr(self):
+        return "%d -> %d, mxfp4%s" % (self.in_features, self.out_features, ", relu" if self.relu else "")
+
+
+def _is_relu(m):
+    return isinstance(m, nn.ReLU) or type(m).__name__ == "_ReLU"
+
+
+def counter_dropout(module, seed):
+    """Replace, IN PLACE, every ``Linear, Dropout(, ReLU)`` run of consecutive children of an ``nn.Sequential`` in ``module`` by ``LinearDropout`` and
+    identities - the places in the sequence, hence the state-dict keys, stay.  -> the number of dropout layers replaced."""
+    count = 0
+    for parent in [m for m in module.modules() if isinstance(m, nn.Sequential)]:
+        names = list(parent._modules)
+        for i in range(len(names) - 1):
+            lin, drop = parent._modules[names[i]], parent._modules[names[i + 1]]
+            if type(lin) is not nn.Linear or type(drop) is not nn.Dropout:
+                continue
+            relu = i + 2 < len(names) and _is_relu(parent._modules[names[i + 2]])
+            parent._modules[names[i]] = LinearDropout(lin, drop.p, layer_seed(seed, count), relu).train(lin.training)
+            parent._modules[names[i + 1]] = nn.Identity().train(lin.training)
+            if relu:
+                parent._modules[names[i + 2]] = nn.Identity().train(lin.training)
+            count += 1
+    return count
+
+
+def mx4_linears(module, prefix=""):
+    """Replace, IN PLACE, every ``nn.Linear`` under ``module`` by ``Mx4LinearLayer`` (a ReLU that follows it in an ``nn.Sequential``, a Dropout between them
+    allowed, runs in its kernel: a dropped or scaled value keeps its sign).  -> [(qualified name, what)]"""
+    done = []
+    for parent_name, parent in list(module.named_modules()):
+        names = list(parent._modules)
+        for i, name in enumerate(names):
+            lin = parent._modules[name]
+            if type(lin) is not nn.Linear:
+                continue
+            at = i + 1
+            if isinstance(parent, nn.Sequential):
+                while at < len(names) and type(parent._modules[names[at]]) in (nn.Dropout, nn.Identity):
+                    at += 1
+            relu = isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
+            parent._modules[name] = Mx4LinearLayer(lin, relu).train(lin.training)
+            if relu:
+                parent._modules[names[at]] = nn.Identity().train(lin.training)
+            done.append((prefix + (parent_name + "." if parent_name else "") + name, "linear %d->%d mxfp4%s" % (lin.in_features, lin.out_features, " + relu" if relu else "")))
+    return done
