@@ -52,6 +52,25 @@ def test_c_calls_refuse_bad_arguments():
     d = lambda x=far(1), c=far(2), s=far(3), rows=3, cols=5, dt=0: lib.adv_mx4_dequantize(c, s, x, rows, cols, dt, None)    # noqa: E731
     for kw in (dict(x=None), dict(dt=-1), dict(x=far(2)), dict(cols=0)):
         assert d(**kw) == _lib.ADV_EINVAL, kw
+    names = ("x", "xc", "xs", "wc", "ws", "bias", "y", "work", "m", "n", "k", "dt", "relu")
+    ok = dict(x=far(1), xc=None, xs=None, wc=far(2), ws=far(3), bias=far(4), y=far(5), work=far(6), m=3, n=4, k=5, dt=0, relu=0)
+    lin = lambda **kw: lib.adv_mx4_linear(*[dict(ok, **kw)[q] for q in names], None)      # noqa: E731
+    for kw in (dict(x=None), dict(xc=far(7)), dict(x=None, xc=far(7)), dict(wc=None), dict(ws=None), dict(y=None), dict(work=None), dict(m=0), dict(n=0), dict(k=0), dict(dt=3),
+               dict(y=far(1)), dict(y=far(2)), dict(y=far(3)), dict(y=far(4)), dict(y=far(6)), dict(work=far(1)), dict(work=far(4)), dict(x=None, xc=far(7), xs=far(5)),
+               dict(m=(1 << 20) + 1), dict(n=(1 << 20) + 1), dict(k=(1 << 20) + 1)):
+        assert lin(**kw) == _lib.ADV_EINVAL, kw
+    for kw in (dict(x=far(1) + 2), dict(wc=far(2) + 8), dict(ws=far(3) + 4), dict(bias=far(4) + 1), dict(y=far(5) + 2), dict(work=far(6) + 128), dict(x=None, xc=far(7) + 8, xs=far(8))):
+        assert lin(**kw) == _lib.ADV_EALIGN, kw
+    assert lib.adv_mx4_linear_workspace_bytes(0, 4, 5) == _lib.ADV_EINVAL and lib.adv_mx4_linear_workspace_bytes(300, 256, 25088) >= 98 * 300 * 136 + 8 * 300 * 256
+    names = ("gy", "mask", "wc", "ws", "gx", "work", "m", "n", "k", "dt")
+    ok = dict(gy=far(1), mask=far(4), wc=far(2), ws=far(3), gx=far(5), work=far(6), m=3, n=4, k=5, dt=0)
+    dg = lambda **kw: lib.adv_mx4_linear_dgrad(*[dict(ok, **kw)[q] for q in names], None)      # noqa: E731
+    for kw in (dict(gy=None), dict(wc=None), dict(ws=None), dict(gx=None), dict(work=None), dict(m=0), dict(n=0), dict(k=0), dict(dt=-1), dict(gx=far(1)), dict(gx=far(4)),
+               dict(gx=far(2)), dict(gx=far(6)), dict(work=far(1)), dict(work=far(4)), dict(work=far(3)), dict(n=1 << 21)):
+        assert dg(**kw) == _lib.ADV_EINVAL, kw
+    for kw in (dict(gy=far(1) + 2), dict(mask=far(4) + 1), dict(wc=far(2) + 4), dict(ws=far(3) + 1), dict(gx=far(5) + 2), dict(work=far(6) + 16)):
+        assert dg(**kw) == _lib.ADV_EALIGN, kw
+    assert lib.adv_mx4_linear_dgrad_workspace_bytes(3, 4, 5, 4) == _lib.ADV_EINVAL and lib.adv_mx4_linear_dgrad_workspace_bytes(3, 4, 5, 0) >= 3 * 3 * 4 * 2
 
 
 def test_ops_refuse_cpu_tensors():
