@@ -160,13 +160,12 @@ __device__ __forceinline__ int by_xcd(int id, int total) {
 
 typedef __attribute__((address_space(3))) void LdsVoid;
 
-// Asks for ROWS 128-byte rows to be copied straight into LDS (16 bytes a lane, lanes in order), swizzled: see staged_chunk.
-// ``at``: this lane's byte offset in the source for each of the ROWS / 32 requests of a thread.
-template <int ROWS>
-__device__ __forceinline__ void stage(const void* base, uint32_t bytes, const uint32_t (&at)[ROWS / 32], uint8_t* lds, int wave) {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
-#pragma unroll
-  for (int j = 0; j < ROWS / 32; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + j * 4096 + wave * 1024), 16, static_cast<int>(at[j]), 0, 0, 0);
+// A panel of a matrix as a buffer resource, and a request for 16 bytes a lane of it straight into LDS (lanes in order from ``lds``)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t panel_of(const uint8_t* base, int p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + static_cast<int64_t>(p) * bytes), 0, static_cast<int>(bytes), 0x00020000);
+}
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t from, uint32_t at, uint8_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsVoid*)lds, 16, static_cast<int>(at), 0, 0, 0);
 }
 
 // 16-byte chunk c of a 128-byte row r lies at chunk c ^ (r / 2 % 8): two rows fill the 64 banks, so the equal chunks of any sixteen neighbouring
@@ -308,20 +307,6 @@ __device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa
 // Many rows: BM x BN of y a workgroup of four waves (2 x 2), 32x32x64 instructions; panels go to LDS by direct copies, two buffers, one barrier a
 // panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is multiplied, and the barrier stands before
 // a panel's last step, whose operands are in registers by then - its products cover the first reads of the next panel.
-// The order of a step's instructions: a wave issues in order and a matrix instruction holds the next one back for its 32 cycles, so what else the
-// step has to issue - READS of LDS, COPIES into it - goes behind its PRODUCTS one by one instead of before them.
-template <int READS, int COPIES, int PRODUCTS>
-__device__ __forceinline__ void weave() {
-  constexpr int kReads = (2 * READS + PRODUCTS - 1) / PRODUCTS, kCopies = (COPIES + PRODUCTS - 1) / PRODUCTS;      // behind one product; reads within the first half
-#pragma unroll
-  for (int k = 0; k < PRODUCTS; ++k) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    if (k * kReads < READS) __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-    if (k * kCopies < COPIES) __builtin_amdgcn_sched_group_barrier(0x010, kCopies, 0);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 template <int BM, int BN>
 constexpr int kTileLds = 2 * (BM + BN) * (128 + 8);
 
@@ -358,21 +343,27 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   const int to_scale = kScales + piece * 1024;
   const uint8_t* scales = for_x ? x.scales : w.scales;
   const uint32_t scale_bytes = (for_x ? x_bytes : w_bytes) >> 4;
-  auto request = [&](int p, int buf) {
-    const int64_t q = p;
-    stage<BM>(x.codes + q * x_bytes, x_bytes, at_x, s_tile + buf * kStage, wave);
-    stage<BN>(w.codes + q * w_bytes, w_bytes, at_w, s_tile + buf * kStage + BM * 128, wave);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales + q * scale_bytes), 0, static_cast<int>(scale_bytes), 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(s_tile + buf * kStage + to_scale), 16, static_cast<int>(at_scale), 0, 0, 0);
+  // copy k of a panel: 32 rows of x's (W's) tile, 8 of them a wave
+  constexpr int kX = BM / 32, kW = BN / 32;
+  uint8_t* const to_x = s_tile + wave * 1024;
+  uint8_t* const to_w = s_tile + BM * 128 + wave * 1024;
+  auto copy_scales = [&](int p, int buf) { copy16(panel_of(scales, p, scale_bytes), at_scale, s_tile + buf * kStage + to_scale); };
+  auto request_x = [&](int p, int buf) {
+    const __amdgpu_buffer_rsrc_t r = panel_of(x.codes, p, x_bytes);
+#pragma unroll
+    for (int k = 0; k < kX; ++k) copy16(r, at_x[k], to_x + buf * kStage + k * 4096);
+  };
+  auto request_w = [&](int p, int buf) {
+    const __amdgpu_buffer_rsrc_t r = panel_of(w.codes, p, w_bytes);
+#pragma unroll
+    for (int k = 0; k < kW; ++k) copy16(r, at_w[k], to_w + buf * kStage + k * 4096);
+    copy_scales(p, buf);
   };
   Uint4 fa[2][TM], fb[2][TN];
-  auto read = [&](int buf, int k, int to) {
-    const uint8_t* a = s_tile + buf * kStage + wm * 128 + frag[k];
-    const uint8_t* b = s_tile + buf * kStage + (BM + wn) * 128 + frag[k];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) fa[to][i] = *reinterpret_cast<const Uint4*>(a + i * 4096);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) fb[to][j] = *reinterpret_cast<const Uint4*>(b + j * 4096);
+  // operand piece i of step k
+  auto read = [&](int buf, int k, int to, int i) {
+    if (i < TM) fa[to][i] = *reinterpret_cast<const Uint4*>(s_tile + buf * kStage + wm * 128 + frag[k] + i * 4096);
+    else fb[to][i - TM] = *reinterpret_cast<const Uint4*>(s_tile + buf * kStage + (BM + wn) * 128 + frag[k] + (i - TM) * 4096);
   };
   uint32_t sx[2][TM], sw[2][TN];
   auto scale_words = [&](int buf, int to) {
@@ -384,37 +375,51 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
     for (int j = 0; j < TN; ++j) sw[to][j] = *reinterpret_cast<const uint32_t*>(b + j * 256);
   };
   Float16 acc[TM][TN] = {};
-#define MX4_STEP(SEL, FROM)                                                                             \
-  _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j)        \
-      acc[i][j] = mfma<SEL>(fa[FROM][i], fb[FROM][j], acc[i][j], sx[0][i], sw[0][j])
-
+  // One step's products, ``also(k)`` behind product k.  A wave issues in order, a product holds the next one back for its 32 cycles, and a copy or a read
+  // that the memory pipes cannot take yet holds back everything behind it: what a step has to ask for goes one by one between its products.
+#define MX4_STEP(SEL, FROM, ALSO)                                                                       \
+  _Pragma("unroll") for (int k = 0; k < TM * TN; ++k) {                                                \
+    acc[k / TN][k % TN] = mfma<SEL>(fa[FROM][k / TN], fb[FROM][k % TN], acc[k / TN][k % TN], sx[0][k / TN], sw[0][k % TN]); \
+    ALSO;                                                                                              \
+    __builtin_amdgcn_sched_barrier(0);                                                                 \
+  }
+  // behind the even products a piece of the next step's operands, behind the odd ones a copy (all of them, should there be fewer products)
+#define READ_NEXT(STEP, TO)                                                                             \
+  _Pragma("unroll") for (int i = 0; i < kReads; ++i)                                                   \
+      if (TM * TN >= 2 * kReads ? i * 2 == k : i * TM * TN / kReads == k) read(buf, STEP, TO, i)
+#define COPY_BETWEEN(COUNT, FROM, AT, TO, BUF)                                                          \
+  _Pragma("unroll") for (int i = 0; i < COUNT; ++i)                                                    \
+      if (TM * TN >= 2 * COUNT ? i * 2 + 1 == k : i * TM * TN / COUNT == k) copy16(FROM, AT[i], TO + (BUF) * kStage + i * 4096)
+  constexpr int kReads = TM + TN;
   // (the tail's requests beyond the last panel ask for that one again, into the buffer nobody reads: one loop body, no branches)
   const int last = end - 1;
-  request(begin, 0);
-  request(min(begin + 1, last), 1);
+  request_x(begin, 0);
+  request_w(begin, 0);
+  request_x(min(begin + 1, last), 1);
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  read(0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) read(0, 0, 0, i);
   scale_words(0, 0);
   int buf = 0;
   for (int p = begin; p < end; ++p) {
-    read(buf, 1, 1);
-    MX4_STEP(0, 0);
-    weave<TM + TN, 0, TM * TN>();
-    read(buf, 2, 0);
-    MX4_STEP(1, 1);
-    weave<TM + TN, 0, TM * TN>();
-    read(buf, 3, 1);
-    MX4_STEP(2, 0);
-    weave<TM + TN, 0, TM * TN>();
+    // x's part of the next panel was asked for in the last step of the one before, W's part is in this step: the copies come evenly
+    const __amdgpu_buffer_rsrc_t rw = panel_of(w.codes, min(p + 1, last), w_bytes), rx = panel_of(x.codes, min(p + 2, last), x_bytes);
+    MX4_STEP(0, 0, {
+      READ_NEXT(1, 1);
+      COPY_BETWEEN(kW, rw, at_w, to_w, buf ^ 1);
+      if (k == TM * TN - 1) copy_scales(min(p + 1, last), buf ^ 1);
+    });
+    MX4_STEP(1, 1, { READ_NEXT(2, 0); });
+    MX4_STEP(2, 0, { READ_NEXT(3, 1); });
     // every wave has this panel's operands in registers, and its copies of the next panel have landed
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    request(min(p + 2, last), buf);
     buf ^= 1;
-    read(buf, 0, 0);
-    scale_words(buf, 1);
-    MX4_STEP(3, 1);
-    weave<2 * (TM + TN), (BM + BN) / 32 + 1, TM * TN>();
+    MX4_STEP(3, 1, {
+      if (k == 0) scale_words(buf, 1);
+      READ_NEXT(0, 0);
+      COPY_BETWEEN(kX, rx, at_x, to_x, buf ^ 1);
+    });
 #pragma unroll
     for (int i = 0; i < TM; ++i) sx[0][i] = sx[1][i];
 #pragma unroll
@@ -422,6 +427,8 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // no copy may land in an LDS that is another workgroup's by then
 #undef MX4_STEP
+#undef READ_NEXT
+#undef COPY_BETWEEN
   float* to = partial + static_cast<int64_t>(part) * x.rows * w.rows;
   const __amdgpu_buffer_rsrc_t out = splits > 1 ? tile_rows(to, m0, x.rows, BM, w.rows * 4) : tile_rows(y, m0, x.rows, BM, w.rows * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
