@@ -6,8 +6,8 @@
 //             A block that holds a NaN or an infinity is NaN as a whole (scale byte 255); an all-zero block has scale byte 0.
 //   linear    y = relu?(Q(x) . W^T + b): a product of two blocks' codes and scales is exact in the matrix instruction, sums are float32
 //   dgrad     gx = (gy where the ReLU let it pass) . W: W's values are exact in bfloat16, and gy goes in as the exact sum of bfloat16 terms
-//             (three for float32, two for half, one for bfloat16) - the contraction runs across W's blocks, which the scaled instruction
-//             cannot do
+//             (three for float32, two for half, one for bfloat16; of a float32 below 2^-110 what lies under 2^-133, bfloat16's last bit, is
+//             cut) - the contraction runs across W's blocks, which the scaled instruction cannot do
 //
 // Layout ("panels" of 256 columns): codes [panel][row][128 bytes], low nibble first; scales [panel][row][8].  What a workgroup reads of a
 // panel - some rows - is one contiguous piece, a lane's scale bytes for four matrix instructions are one aligned dword, and a panel is
@@ -29,7 +29,6 @@ typedef float Float16 __attribute__((ext_vector_type(16)));
 typedef float Float2 __attribute__((ext_vector_type(2)));
 typedef float Float4 __attribute__((ext_vector_type(4)));
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t Uint2 __attribute__((ext_vector_type(2)));
 typedef uint32_t Uint4 __attribute__((ext_vector_type(4)));
 
 __host__ __device__ inline int64_t panels_of(int64_t cols) { return (cols + kPanel - 1) / kPanel; }
@@ -201,7 +200,7 @@ __device__ __forceinline__ void put_tile(__amdgpu_buffer_rsrc_t to, const Float1
 // Few rows of x: bound by reading W once.  16 rows of W (A) x 16 * MT rows of x (B) a workgroup on 16x16x128 instructions, operands straight
 // from memory to registers (a panel's 16 rows are 2 KB in one piece); the waves share the panels out and join their sums in LDS, in order.
 // RAW: x comes as values (four rows at most); every workgroup quantises them for itself into LDS while its first piece of W is on its way - a second
-// reading of x from the L2 for every 16 rows of W, against a launch of its own (17.0 -> 13.6 us for one crop).
+// reading of x from the L2 for every 16 rows of W, against a launch of its own: one row of 25088 x 4096 18.1 -> 15.3 us, of 4096 x 1000 12.1 -> 9.9.
 template <class T, int MT, bool RAW>
 __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __restrict__ values, int64_t cols, Operand w, const T* __restrict__ bias, T* __restrict__ y,
                                                        int panels, int relu) {
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __res
   Float4 acc[MT] = {};
 #pragma unroll
   for (int i = 0; i < MT; ++i) m[i] = min(m0 + 16 * i + (lane & 15), x.rows - 1);
-  constexpr int U = MT == 1 ? 4 : 2;                                   // panels whose operands are on their way together
+  constexpr int U = MT == 1 && !RAW ? 4 : 2;                           // panels whose operands are on their way together (RAW: the others' registers hold x)
   Uint4 a[U][2];
   uint32_t sa[U];
   auto fetch = [&](int p0) {
@@ -375,7 +374,7 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
     for (int j = 0; j < TN; ++j) sw[to][j] = *reinterpret_cast<const uint32_t*>(b + j * 256);
   };
   Float16 acc[TM][TN] = {};
-  // One step's products, ``also(k)`` behind product k.  A wave issues in order, a product holds the next one back for its 32 cycles, and a copy or a read
+  // One step's products, ALSO behind product k.  A wave issues in order, a product holds the next one back for its 32 cycles, and a copy or a read
   // that the memory pipes cannot take yet holds back everything behind it: what a step has to ask for goes one by one between its products.
 #define MX4_STEP(SEL, FROM, ALSO)                                                                       \
   _Pragma("unroll") for (int k = 0; k < TM * TN; ++k) {                                                \
@@ -493,7 +492,7 @@ constexpr int kTerms = sizeof(T) == 4 ? 3 : 2;
 template <>
 constexpr int kTerms<__bf16> = 1;
 
-// v as the exact sum of N bfloat16 (cut, not rounded: what is left always fits the next ones, and a finite v stays finite)
+// v as the sum of N bfloat16, exact but for bits under 2^-133 (cut, not rounded: what is left always fits the next ones, and a finite v stays finite)
 template <int N>
 __device__ __forceinline__ void split(float v, uint32_t (&t)[N]) {
   const uint32_t u = __float_as_uint(v);

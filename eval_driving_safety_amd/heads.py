@@ -16,7 +16,8 @@ def layer_seed(seed, index):
 
 class LinearDropout(nn.Linear):
     """``relu?(dropout(linear(x)))`` with ``nn.Linear``'s parameters and state-dict keys.  In training every forward takes the next ``step`` (a plain
-    number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device."""
+    number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device.  For a step captured in a
+    hipGraph set ``step`` to an int64 CUDA tensor of one element and move it on between the replays (a number would repeat one mask: refused)."""
 
     def __init__(self, linear, p, seed, relu=False):
         nn.Module.__init__(self)
@@ -29,8 +30,14 @@ class LinearDropout(nn.Linear):
             y = F.linear(x, self.weight, self.bias)
             return F.relu(y) if self.relu else y
         from . import ops
-        step, self.step = self.step, self.step + 1
-        return ops.Dropout.apply(F.linear(x, self.weight), self.p, self.seed, step, self.bias, self.relu)
+        step = self.step
+        if not isinstance(step, torch.Tensor):
+            if x.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("LinearDropout: a captured step needs `step` as an int64 CUDA tensor (a number would give every replay the same mask)")
+            self.step = step + 1
+        y = F.linear(x, self.weight).contiguous()
+        bias = self.bias if self.bias is None or self.bias.dtype == y.dtype else self.bias.to(y.dtype)      # (under autocast the product's type)
+        return ops.Dropout.apply(y, self.p, self.seed, step, bias, self.relu)
 
     def extra_repr(self):
         return "%s, p=%g, seed=%d, relu=%s" % (nn.Linear.extra_repr(self), self.p, self.seed, self.relu)
@@ -38,7 +45,7 @@ class LinearDropout(nn.Linear):
 
 class Mx4LinearLayer(nn.Module):
     """``relu?(linear(x))`` with the weight in MXFP4 and x quantised on the way in; the weight is quantised when the layer first runs on a ROCm device
-    (its float32 copy is given up then)"""
+    (its float copy is given up then: code that reads the layer's ``weight`` does not work on it)"""
 
     def __init__(self, linear, relu=False):
         super().__init__()
@@ -54,6 +61,8 @@ class Mx4LinearLayer(nn.Module):
         if self.codes is None:
             if not self.weight.is_cuda:
                 raise RuntimeError("Mx4LinearLayer: libadvengine has no CPU path - move the model and its inputs to the ROCm device")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Mx4LinearLayer: run the layer once before capturing it (its weight is quantised on first use)")
             q = ops.mx4_quantize(self.weight.contiguous())
             self.codes, self.scales, self.weight = q.codes, q.scales, None
         return ops.Mx4(self.codes, self.scales, (self.out_features, self.in_features))

@@ -110,8 +110,8 @@ def mx4_linear(x, w, bias=None, relu=False, dtype=None):
 
 def mx4_linear_dgrad(grad_y, w, mask=None):
     """the gradient of ``mx4_linear`` w.r.t. ``x`` -> [..., K], straight through x's quantisation (adv_mx4_linear_dgrad): ``(grad_y where mask > 0) . W``
-    with ``mask`` the layer's output where it had a ReLU, else None.  ``grad_y`` [..., N] float32 / bfloat16 / float16 enters exactly; sums are
-    float32."""
+    with ``mask`` the layer's output where it had a ReLU, else None.  ``grad_y`` [..., N] float32 / bfloat16 / float16 enters exactly (bits of a float32 under
+    2**-133 are cut); sums are float32."""
     _mx4(w, "w")
     _head(grad_y, "grad_y")
     if len(w.shape) != 2 or grad_y.dim() < 1 or grad_y.shape[-1] != w.rows:

@@ -655,8 +655,8 @@ ADV_API int adv_dropout_bwd(const void* gy, const void* y, void* gx, void* gbias
  *               holds a NaN or an infinity gets scale byte 255: it is NaN as a whole.
  *   _linear     y [m, n] = relu?(X . W^T + bias) for X [m, k] and W [n, k] in MXFP4, bias [n] or NULL; products exact, sums float32.  X comes as
  *               values x [m, k] of type `dtype` (then x_codes = x_scales = NULL: quantised on the way), or as x_codes / x_scales (then x = NULL).
- *   _linear_dgrad  gx [m, k] = G . W, G [m, n] = gy, 0 where mask (NULL, or laid out like gy: the layer's ReLU output) is <= 0; gy enters exactly,
- *               sums float32.
+ *   _linear_dgrad  gx [m, k] = G . W, G [m, n] = gy, 0 where mask (NULL, or laid out like gy: the layer's ReLU output) is <= 0; gy enters exactly
+ *               (bits of a float32 under 2^-133 are cut), sums float32.
  *   workspace   device memory of _workspace_bytes bytes, 256-byte aligned, not shared with a call that may run at the same time.
  *   The order of the additions depends on the sizes alone: the same call gives the same bits. */
 ADV_API int64_t adv_mx4_code_bytes(int64_t rows, int64_t cols);

@@ -108,6 +108,53 @@ def test_two_runs_train_to_the_same_weights_whatever_the_generator(tmp_path):
 
 
 @pytest.mark.gpu
+def test_captured_layers_take_a_step_tensor_and_a_quantised_weight():
+    h = small_head(6).cuda()
+    heads.counter_dropout(h, 3)
+    l1 = h[1].train()
+    x = torch.randn(9, 72, generator=torch.Generator().manual_seed(3)).cuda()
+    q = nn.Sequential(nn.Linear(72, 8)).cuda()
+    heads.mx4_linears(q)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm), torch.no_grad():
+        l1(x)
+    torch.cuda.current_stream().wait_stream(warm)
+    for layer in (l1, q):                                 # a number as step, a weight not yet quantised: refused, nothing is captured
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="captur"):
+            with torch.cuda.graph(graph):
+                x.add(1)
+                layer(x)
+        torch.cuda.synchronize()
+    l1.step = torch.zeros((1,), dtype=torch.int64, device="cuda")
+    with torch.no_grad():
+        q(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, z = l1(x), q(x)
+        for k in (5, 6, 7):
+            l1.step.fill_(k)
+            graph.replay()
+            torch.cuda.synchronize()
+            a = F.linear(x, l1.weight).double().cpu().numpy()
+            np.testing.assert_allclose(y.cpu().numpy(), O.dropout(a, 0.1, l1.seed, k, l1.bias.double().cpu().numpy(), True), rtol=1e-6, atol=1e-6)
+            assert torch.equal(z, q(x))
+
+
+@pytest.mark.gpu
+def test_training_under_autocast():
+    h = small_head(7).cuda()
+    heads.counter_dropout(h, 4)
+    h.train()
+    x = torch.randn(5, 72, generator=torch.Generator().manual_seed(4)).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = h(x)
+    y.float().sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all() for p in h.parameters())
+
+
+@pytest.mark.gpu
 def test_quantised_head_validates_and_carries_the_image_gradient():
     """eval with four-bit weights against the same layers on the values those bits hold, in float64; the gradient w.r.t. the input straight through"""
     h = small_head(4).eval().cuda()

@@ -258,6 +258,15 @@ def test_hip_blocks_without_a_value_and_extreme_scales():
     g = torch.tensor([[3.4e38, -3.4e38, 1.1754944e-38, 1e-30]], device="cuda")
     wt = torch.tensor(np.eye(4, 40, dtype=np.float32)).cuda()
     assert torch.equal(ops.mx4_linear_dgrad(g, ops.mx4_quantize(wt))[:, :4], g)
+    # gradients whose last bits lie under 2^-133: those are cut, each off by less than that
+    g = make((3, 20), torch.float32, 6) * 2.0 ** -125
+    q = ops.mx4_quantize(make((20, 64), torch.float32, 7) * 2.0 ** 100)
+    wv = np64(q.dequantize())
+    d = np.abs(np64(ops.mx4_linear_dgrad(g, q)) - np64(g) @ wv)
+    assert (d <= 2.0 ** -133 * np.abs(wv).sum(0) + (20 / 8 * 3 + 16) * 2.0 ** -23 * (np.abs(np64(g)) @ np.abs(wv))).all()
+    # products of subnormals are not flushed
+    a, b = torch.full((2, 64), 2.0 ** -100, device="cuda"), torch.full((5, 64), 2.0 ** -36, device="cuda")
+    assert (np64(ops.mx4_linear(a, ops.mx4_quantize(b))) == 64 * 2.0 ** -136).all()
 
 
 @pytest.mark.gpu
