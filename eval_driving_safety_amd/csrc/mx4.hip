@@ -581,16 +581,11 @@ __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uin
   }
   const uint8_t* plane0 = planes + m0 * padded * 2;
   const uint32_t tile_bytes = static_cast<uint32_t>(min(static_cast<int64_t>(BM), rows - m0) * padded * 2);
-  auto request = [&](int c, int buf) {
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(plane0 + s * rows * padded * 2 + static_cast<int64_t>(c) * (kChunk * 2)), 0,
-                                                                         static_cast<int>(tile_bytes - static_cast<uint32_t>(c) * (kChunk * 2)), 0x00020000);
-#pragma unroll
-      for (int j = 0; j < kCopies; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(s_g + (buf * N + s) * kTermBytes + j * 4096 + (BM >= 64 ? wave : wave & 1) * 1024), 16, static_cast<int>(at[j]), 0,
-                                                 0, 0);
-    }
+  auto copy = [&](int c, int buf, int e) {             // copy e of a chunk: kCopies of each term
+    const int s = e / kCopies, j = e % kCopies;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(plane0 + s * rows * padded * 2 + static_cast<int64_t>(c) * (kChunk * 2)), 0,
+                                                                       static_cast<int>(tile_bytes - static_cast<uint32_t>(c) * (kChunk * 2)), 0x00020000);
+    copy16(r, at[j], s_g + (buf * N + s) * kTermBytes + j * 4096 + (BM >= 64 ? wave : wave & 1) * 1024);
   };
 
   // 32 columns - one block - of one row of W a thread; rows behind the last one read as zeros (the resource ends there): the value 0 under the scale 2^-127
@@ -609,10 +604,9 @@ __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uin
     h.scale = __builtin_amdgcn_raw_buffer_load_b8(rs, t, 0, 0);
   };
   const uint32_t put_at = static_cast<uint32_t>(wide_row(t >> 3, (t & 7) * 4));
-  auto turn = [&](const Held& h, int buf) {
+  auto turn = [&](const Held& h, int buf, int k) {     // a quarter of it: eight columns
     const float f = __uint_as_float(h.scale << 23);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    {
       Uint4 out;
       out[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 0));
       out[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(h.code[k], f, 1));
@@ -639,41 +633,47 @@ __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uin
       }
     }
   };
-  auto multiply = [&](int buf, const Bf16x8 (&b)[K][TJ]) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int s = 0; s < N; ++s) {
-#pragma unroll
-        for (int i = 0; i < TI; ++i) {
-          const Bf16x8 a = *reinterpret_cast<const Bf16x8*>(read_g + (place_g ^ static_cast<uint32_t>(k * 32)) + (buf * N + s) * kTermBytes + i * 2048);
-#pragma unroll
-          for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[k][j], acc[i][j], 0, 0, 0);
-        }
-      }
-    }
+  constexpr int kFrags = K * N * TI;                   // gy's operands of a chunk, in order of use: k, term, row block
+  auto frag = [&](int buf, int e) {
+    const int k = e / (N * TI), s = e / TI % N, i = e % TI;
+    return *reinterpret_cast<const Bf16x8*>(read_g + (place_g ^ static_cast<uint32_t>(k * 32)) + (buf * N + s) * kTermBytes + i * 2048);
   };
 
   Held held[kHeld];                                    // chunk c is in held[c % kHeld]
-  request(begin, 0);
+#pragma unroll
+  for (int e = 0; e < N * kCopies; ++e) copy(begin, 0, e);
   __builtin_amdgcn_sched_barrier(0);                   // (the copies must be older than the two loads that step() leaves on their way)
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) fetch(min(begin + k, last), held[k]);
-  turn(held[0], 0);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) turn(held[0], 0, k);
   fetch(min(begin + kHeld, last), held[0]);
-  auto step = [&](int c, Held& h, int buf) {           // h: holds chunk c + 1, is given chunk c + 1 + kHeld
+  // h: holds chunk c + 1, is given chunk c + 1 + kHeld.  Everything a step asks for or converts goes between its products, in a fixed order: gy's
+  // operands two groups of products ahead, then the copies, then the four quarters of the next chunk of W, then its loads.
+  constexpr int kExtras = N * kCopies + 5;
+  auto step = [&](int c, Held& h, int buf) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // chunk c's copies have landed: only the two loads of chunk c + kHeld came after
-    Bf16x8 b[K][TJ];
+    Bf16x8 b[K][TJ], g[kFrags];
     read(buf, b);                                      // before the next copies are asked for: the compiler takes a turned read to depend on every copy on its way
+    g[0] = frag(buf, 0);
+    if (kFrags > 1) g[1] = frag(buf, 1);
     __builtin_amdgcn_sched_barrier(0);
-    request(min(c + 1, last), buf ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
-    turn(h, buf ^ 1);
-    fetch(min(c + 1 + kHeld, last), h);
-    __builtin_amdgcn_s_setprio(1);                     // a wave that multiplies goes before its neighbour's conversions: 159 -> 150 us for 512 rows
-    multiply(buf, b);
-    __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+    for (int e = 0; e < kFrags; ++e) {
+      if (e + 2 < kFrags) g[e + 2] = frag(buf, e + 2);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[e % TI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g[e], b[e / (N * TI)][j], acc[e % TI][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < kExtras; ++x) {
+        if (x * kFrags / kExtras != e) continue;
+        if (x < N * kCopies) copy(min(c + 1, last), buf ^ 1, x);
+        else if (x < N * kCopies + 4) turn(h, buf ^ 1, x - N * kCopies);
+        else fetch(min(c + 1 + kHeld, last), h);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   };
   for (int c = begin; c < end; c += kHeld) {           // (chunks come in fours: the planes are padded to them)
 #pragma unroll
