@@ -185,7 +185,7 @@ def close_product(got, a, b, dtype, bias, relu, per_step, what):
 
 
 LINEAR = [(1, 1, 1), (1, 32, 64), (2, 33, 31), (1, 4096, 2048), (16, 100, 257), (17, 31, 1000), (33, 65, 512), (64, 300, 25088), (65, 257, 1999), (130, 129, 4100),
-          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96)]
+          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96), (2050, 4100, 300), (2047, 4090, 2100)]
 
 
 @pytest.mark.gpu
