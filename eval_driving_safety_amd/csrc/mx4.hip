@@ -199,7 +199,7 @@ __device__ __forceinline__ void put_tile(__amdgpu_buffer_rsrc_t to, const Float1
 
 // Few rows of x: bound by reading W once.  16 rows of W (A) x 16 * MT rows of x (B) a workgroup on 16x16x128 instructions, operands straight
 // from memory to registers (a panel's 16 rows are 2 KB in one piece); the waves share the panels out and join their sums in LDS, in order.
-// RAW: x comes as values (four rows at most); every workgroup quantises them for itself into LDS while its first piece of W is on its way - a second
+// RAW: x comes as values (few of them: thin_raw); every workgroup quantises them for itself into LDS while its first piece of W is on its way - a second
 // reading of x from the L2 for every 16 rows of W, against a launch of its own: one row of 25088 x 4096 18.1 -> 15.3 us, of 4096 x 1000 12.1 -> 9.9.
 template <class T, int MT, bool RAW>
 __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __restrict__ values, int64_t cols, Operand w, const T* __restrict__ bias, T* __restrict__ y,
@@ -759,8 +759,11 @@ void run_join(const float* partial, const void* bias, void* y, int64_t rows, int
 
 constexpr int kThinLds = 64 * 1024;        // a workgroup's share: two on a CU
 int thin_waves(int panels) { return panels >= 16 ? 8 : (panels >= 4 ? 4 : 1); }
-// the rows of x fit a thin workgroup's LDS in four bits
-bool thin_raw(int64_t m, int64_t k) { return m <= 4 && panels_of(k) * m * 136 + 8 * 1024 <= kThinLds; }
+// x is quantised inside the thin product: up to four rows, and up to 16 of 128 KB together, where they fit a workgroup's LDS in four bits. 8 rows of
+// 4096 float32: 10.3 against 12.9 us with a launch of its own; 16 rows of 2048: 12.7 against 12.6, the break-even; of 4096: 14.4 against 12.6.
+bool thin_raw(int64_t m, int64_t k, int bytes) {
+  return (m <= 4 || (m <= 16 && m * k * bytes <= 128 * 1024)) && panels_of(k) * m * 136 + 8 * 1024 <= kThinLds;
+}
 
 template <class T, int MT, bool RAW>
 int run_thin(Operand x, const void* values, int64_t k, Operand w, const void* bias, void* y, int relu, hipStream_t st) {
@@ -785,7 +788,7 @@ int run_tile(Operand x, Operand w, const void* bias, void* y, float* partial, in
 template <class T>
 int run_linear(Operand x, const void* values, Operand w, const void* bias, void* y, uint8_t* ws, int64_t k, int relu, hipStream_t st) {
   const LinearPlan p = plan_linear(x.rows, w.rows, k);
-  if (!x.codes && p.thin && thin_raw(x.rows, k)) return run_thin<T, 1, true>(x, values, k, w, bias, y, relu, st);
+  if (!x.codes && p.thin && thin_raw(x.rows, k, static_cast<int>(sizeof(T)))) return run_thin<T, 1, true>(x, values, k, w, bias, y, relu, st);
   const int64_t cb = padded(code_bytes(x.rows, k)), sb = padded(scale_bytes(x.rows, k));
   if (!x.codes) {
     const int bad = run_quantize<T>(values, ws, ws + cb, x.rows, k, st);
