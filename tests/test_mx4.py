@@ -166,6 +166,20 @@ def test_hip_unaligned_rows_and_offsets_beyond_32_bits():
     assert torch.allclose(gx, gs, rtol=0, atol=8 * 2.0 ** -23 * float(gs.abs().max() + gt.abs().max() * tail.abs().max() * 5))
 
 
+@pytest.mark.gpu
+def test_hip_gradient_of_more_rows_than_a_launch_is_wide():
+    from eval_driving_safety_amd import ops
+    m, n, k = 66000, 2048, 32                              # 2^24 threads and some more, eight of a row each
+    g, w = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda"), make((n, k), torch.float32, 2)
+    at = torch.tensor([0, 63, 8191, 32767, 65535, 65536, 65537, 65999], device="cuda")
+    g[at] = make((len(at), n), torch.bfloat16, 1)
+    q = ops.mx4_quantize(w)
+    gx = ops.mx4_linear_dgrad(g, q)
+    close_product(gx[at], np64(g[at]), np64(q.dequantize()), torch.bfloat16, None, False, 8.0, "tall gradient")
+    gx[at] = 0
+    assert not gx.any()
+
+
 # ---------------------------------------------------------------------------------------------------------------- products
 def close_product(got, a, b, dtype, bias, relu, per_step, what):
     """got against relu?(a @ b + bias) in float64, a [M,K], b [K,N].  Each float32 addition of a running sum is off by at most one unit in the last
@@ -185,7 +199,7 @@ def close_product(got, a, b, dtype, bias, relu, per_step, what):
 
 
 LINEAR = [(1, 1, 1), (1, 32, 64), (2, 33, 31), (1, 4096, 2048), (16, 100, 257), (17, 31, 1000), (33, 65, 512), (64, 300, 25088), (65, 257, 1999), (130, 129, 4100),
-          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96), (2050, 4100, 300), (2047, 4090, 2100)]
+          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96), (2050, 4100, 300), (2047, 4090, 2100), (8, 40, 4096), (9, 70, 4097), (16, 50, 2048), (16, 90, 4000), (5, 1000, 6500), (13, 20, 16)]
 
 
 @pytest.mark.gpu
