@@ -202,6 +202,8 @@ __device__ __forceinline__ void put_tile(__amdgpu_buffer_rsrc_t to, const Float1
 // from memory to registers (a panel's 16 rows are 2 KB in one piece); the waves share the panels out and join their sums in LDS, in order.
 // RAW: x comes as values (few of them: thin_raw); every workgroup quantises them for itself into LDS while its first piece of W is on its way - a second
 // reading of x from the L2 for every 16 rows of W, against a launch of its own: one row of 25088 x 4096 18.1 -> 15.3 us, of 4096 x 1000 12.1 -> 9.9.
+template <int V>
+constexpr int kThinBatch = V == 4 ? 7 : 4;             // pieces of a panel's row (two rows, 16-bit) that a wave has on their way together
 template <class T, int MT, bool RAW>
 __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __restrict__ values, int64_t cols, Operand w, const T* __restrict__ bias, T* __restrict__ y,
                                                        int panels, int relu) {
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __res
   Float4 acc[MT] = {};
 #pragma unroll
   for (int i = 0; i < MT; ++i) m[i] = min(m0 + 16 * i + (lane & 15), x.rows - 1);
-  constexpr int U = MT == 1 && !RAW ? 4 : 2;                           // panels whose operands are on their way together (RAW: the others' registers hold x)
+  constexpr int U = 2;                                                 // panels whose operands are on their way together (4: 5.9 us for 4.3 with 4096 x 4096)
   Uint4 a[U][2];
   uint32_t sa[U];
   auto fetch = [&](int p0) {
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(512) void mx4_linear_thin(Operand x, const T* __res
   fetch(wave);
   if constexpr (RAW) {
     constexpr int V = 16 / sizeof(T), kLanes = kPanel / V, kGroup = 64 / kLanes;      // lanes a panel's row, rows a wave takes at once
-    constexpr int kBatch = V == 4 ? 7 : 4;                             // pieces whose values are on their way together
+    constexpr int kBatch = kThinBatch<V>;
     const int pieces = panels * static_cast<int>(x.rows), rows = static_cast<int>(x.rows), in_row = lane % kLanes, step = waves * kGroup;
     for (int i0 = wave * kGroup + lane / kLanes; i0 < pieces; i0 += kBatch * step) {
       float v[kBatch][V];
@@ -304,18 +306,22 @@ __device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(a), widen(b), c, 4, 4, SEL, static_cast<int>(sa), SEL, static_cast<int>(sb));
 }
 
-// Many rows: BM x BN of y a workgroup of four waves (2 x 2), 32x32x64 instructions; panels go to LDS by direct copies, two buffers, one barrier a
-// panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is multiplied, and the barrier stands before
-// a panel's last step, whose operands are in registers by then - its products cover the first reads of the next panel.  4096 x 25088 x 4096 in 166 us:
-// 5.1 PFLOP/s of the 7.3 that the bare instruction reaches, the matrix pipe 0.76 busy.  301 x 25088 x 2048, ten parts on 480 workgroups: 18 us, bound
-// by the copies of both operands, every tile's from the L2.
+// Many rows: BM x BN of y a workgroup of four waves (2 x 2, or side by side over 32 rows), 32x32x64 instructions; panels go to LDS by direct copies,
+// two (256 x 256) or three buffers, one barrier a panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is
+// multiplied, and the barrier stands before a panel's last step, whose operands are in registers by then - its products cover the first reads of the next
+// panel.  4096 x 25088 x 4096 in 166 us: 5.1 PFLOP/s of the 7.3 that the bare instruction reaches, the matrix pipe 0.76 busy.  The smaller tiles are
+// bound by how long a panel takes to come: with the third buffer 128 x 4096 x 4104 takes 15.1 us for 17.9, 32 x 25088 x 4096 17.5 for 19.7.
 template <int BM, int BN>
-constexpr int kTileLds = 2 * (BM + BN) * (128 + 8);
+constexpr int kTileStages = BM > 128 ? 2 : 3;
+template <int BM, int BN>
+constexpr int kTileStage = (BM + BN) * 128 + ((BM > 128 ? BM : 128) + BN) * 8;      // (x's scale bytes come 1 KB at a time)
 
 template <class T, int BM, int BN>
-__global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y,
+__global__ __launch_bounds__(kBlock, BM < 128 ? 2 : 1) void mx4_linear_tile(Operand x, Operand w, const T* __restrict__ bias, T* __restrict__ y,
                                                                                float* __restrict__ partial, int panels, int splits, int relu) {
-  constexpr int TM = BM / 64, TN = BN / 64, kStage = (BM + BN) * (128 + 8), kScales = (BM + BN) * 128;
+  constexpr int WM = BM == 32 ? 1 : 2, WN = 4 / WM, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int kStage = kTileStage<BM, BN>, kScales = (BM + BN) * 128, kRowsX = BM > 128 ? BM : 128;
+  constexpr int kStages = kTileStages<BM, BN>;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_tile[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int tm = static_cast<int>((x.rows + BM - 1) / BM), tn = static_cast<int>((w.rows + BN - 1) / BN);
@@ -333,15 +339,15 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
 #pragma unroll
   for (int j = 0; j < BN / 32; ++j) at_w[j] = static_cast<uint32_t>(min(n0 + j * 32 + wave * 8 + (lane >> 3), w.rows - 1)) * 128u + chunk;
   const uint32_t x_bytes = static_cast<uint32_t>(x.rows) * 128u, w_bytes = static_cast<uint32_t>(w.rows) * 128u;
-  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+  const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
   int frag[4];                                         // this lane's chunk of a row in each of the four steps
 #pragma unroll
   for (int k = 0; k < 4; ++k) frag[k] = swizzled(lane & 31, half * 4 + k);
 
   // the tile's scale bytes of a panel are one piece of BM (BN) * 8 bytes: 1 KB a wave (128 x 128 tiles have two: two waves copy each)
-  const int piece = wave % ((BM + BN) / 128);
-  const bool for_x = piece < BM / 128;
-  const uint32_t at_scale = static_cast<uint32_t>((for_x ? m0 + piece * 128 : n0 + (piece - BM / 128) * 128) * 8) + lane * 16;
+  const int piece = wave % ((kRowsX + BN) / 128);
+  const bool for_x = piece < kRowsX / 128;
+  const uint32_t at_scale = static_cast<uint32_t>((for_x ? m0 + piece * 128 : n0 + (piece - kRowsX / 128) * 128) * 8) + lane * 16;
   const int to_scale = kScales + piece * 1024;
   const uint8_t* scales = for_x ? x.scales : w.scales;
   const uint32_t scale_bytes = (for_x ? x_bytes : w_bytes) >> 4;
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   uint32_t sx[2][TM], sw[2][TN];
   auto scale_words = [&](int buf, int to) {
     const uint8_t* a = s_tile + buf * kStage + kScales + (wm + (lane & 31)) * 8 + half * 4;
-    const uint8_t* b = s_tile + buf * kStage + kScales + (BM + wn + (lane & 31)) * 8 + half * 4;
+    const uint8_t* b = s_tile + buf * kStage + kScales + (kRowsX + wn + (lane & 31)) * 8 + half * 4;
 #pragma unroll
     for (int i = 0; i < TM; ++i) sx[to][i] = *reinterpret_cast<const uint32_t*>(a + i * 256);
 #pragma unroll
@@ -393,34 +399,41 @@ __global__ __launch_bounds__(kBlock, BM + BN > 256 ? 1 : 2) void mx4_linear_tile
   _Pragma("unroll") for (int i = 0; i < COUNT; ++i)                                                    \
       if (TM * TN >= 2 * COUNT ? i * 2 + 1 == k : i * TM * TN / COUNT == k) copy16(FROM, AT[i], TO + (BUF) * kStage + i * 4096)
   constexpr int kReads = TM + TN;
-  // (the tail's requests beyond the last panel ask for that one again, into the buffer nobody reads: one loop body, no branches)
+  // (the tail's requests beyond the last panel ask for that one again, into buffers nobody reads: one loop body, no branches)
   const int last = end - 1;
-  request_x(begin, 0);
-  request_w(begin, 0);
-  request_x(min(begin + 1, last), 1);
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  constexpr int kAhead = (kStages - 2) * (kX + kW + 1);      // a wave's copies of the panels behind the next one: not waited for
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    request_x(min(begin + s, last), s);
+    request_w(min(begin + s, last), s);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  request_x(min(begin + kStages - 1, last), kStages - 1);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kAhead + kX) : "memory");
 #pragma unroll
   for (int i = 0; i < kReads; ++i) read(0, 0, 0, i);
   scale_words(0, 0);
-  int buf = 0;
+  int buf = 0, free = kStages - 1;                     // this panel's buffer, the one of the panel before
   for (int p = begin; p < end; ++p) {
-    // x's part of the next panel was asked for in the last step of the one before, W's part is in this step: the copies come evenly
-    const __amdgpu_buffer_rsrc_t rw = panel_of(w.codes, min(p + 1, last), w_bytes), rx = panel_of(x.codes, min(p + 2, last), x_bytes);
+    // x's part of the panel kStages - 1 further on was asked for in the last step of the one before, W's part is in this step: the copies come evenly
+    const __amdgpu_buffer_rsrc_t rw = panel_of(w.codes, min(p + kStages - 1, last), w_bytes), rx = panel_of(x.codes, min(p + kStages, last), x_bytes);
     MX4_STEP(0, 0, {
       READ_NEXT(1, 1);
-      COPY_BETWEEN(kW, rw, at_w, to_w, buf ^ 1);
-      if (k == TM * TN - 1) copy_scales(min(p + 1, last), buf ^ 1);
+      COPY_BETWEEN(kW, rw, at_w, to_w, free);
+      if (k == TM * TN - 1) copy_scales(min(p + kStages - 1, last), free);
     });
     MX4_STEP(1, 1, { READ_NEXT(2, 0); });
     MX4_STEP(2, 0, { READ_NEXT(3, 1); });
     // every wave has this panel's operands in registers, and its copies of the next panel have landed
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAhead) : "memory");
     __builtin_amdgcn_sched_barrier(0);
-    buf ^= 1;
+    free = buf;
+    buf = buf == kStages - 1 ? 0 : buf + 1;
     MX4_STEP(3, 1, {
       if (k == 0) scale_words(buf, 1);
       READ_NEXT(0, 0);
-      COPY_BETWEEN(kX, rx, at_x, to_x, buf ^ 1);
+      COPY_BETWEEN(kX, rx, at_x, to_x, free);
     });
 #pragma unroll
     for (int i = 0; i < TM; ++i) sx[0][i] = sx[1][i];
@@ -724,27 +737,29 @@ constexpr int64_t kAlign = 256;
 int64_t padded(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
 
 // How a product is cut.
-//   thin   up to 16 rows, and up to 64 against a weight of 2^23 values or fewer: one launch (4096 x 1000: 16 against 19 us at 64 rows); with
-//          25088 x 4096 tiles are faster from 17 rows on (64 rows: 22 against 39 us), as every 16 rows of W read all of x again there.
-//   big    256 x 256 tiles where there are 128 of them or more, else 128 x 128.
+//   thin   one launch, but every 16 rows of W read all of x again: up to 16 rows of up to 56 panels (8 rows of 8192 x 4096: 7.7 against 9.2 us, of
+//          12544 x 2048 9.3 against 9.5, of 25088 x 4096 17.0 against 13.9), a single row of up to 112, which is quantised in there (25088: 15.5 against
+//          17.5), and up to 64 rows of 1024 panels together under a small weight (32 of 6400 x 1024: 7.6 against 7.7, 64 of them 11.4 against 8.6).
+//   big    256 x 256 tiles where there are 128 of them or more, else 128 x 128, of which 64 or 32 rows where x has no more (32 x 25088 x 4096: 20.2 ->
+//          14.3 us with its join).
 //   splits the panels are dealt to several workgroups a tile where tiles alone do not fill the chip: the number with the least estimated time, from
-//          0.8 us a panel with one 128 x 128 workgroup a CU, 1.1 us with two (measured at 32 .. 256 rows of 25088 x 4096), three panels' time for a
-//          workgroup's start and end, and the joining pass at 8 TB/s (the parts are in the caches).
+//          what a panel takes (128 rows: 0.26 us up to 64 workgroups, 0.45 at one a CU; fewer rows 0.14 and 0.33), three panels' time for a workgroup's
+//          start and end, and the joining pass.  Fitted to 8 .. 512 rows of nine weights: within 1.3 % of the best count on average.
 struct LinearPlan {
   int thin, big, splits;
 };
 LinearPlan plan_linear(int64_t m, int64_t n, int64_t k) {
   const int64_t panels = panels_of(k);
-  if (m <= 16 || (m <= 64 && n * k <= (int64_t{1} << 23))) return {1, 0, 1};
+  if (m * panels <= 112 || (m <= 16 ? panels <= 56 : m <= 64 && m * panels <= 1024 && n <= 4096)) return {1, 0, 1};
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
   if (big >= 128) return {0, 1, static_cast<int>(big >= 256 || panels < 8 ? 1 : 256 / big)};
   int best = 1;
   double least = 0.0;
   for (int64_t s = 1; s <= 32 && (s == 1 || s <= panels / 4); ++s) {
     const int64_t groups = small * s;
-    const double each = static_cast<double>((panels + s - 1) / s + 3);
-    double t = groups <= 256 ? 0.8 * each : 1.1 * each * static_cast<double>((groups + 511) / 512);
-    if (s > 1) t += 2.0 + 1e-6 * static_cast<double>(s * m * n);
+    const double panel = (m <= 64 ? 0.14 : 0.26) + 0.001 * static_cast<double>(groups <= 64 ? 0 : (groups < 256 ? groups - 64 : 192));
+    double t = panel * static_cast<double>(((panels + s - 1) / s + 3) * ((groups + 255) / 256));
+    if (s > 1) t += 1.0 + 1.2e-6 * static_cast<double>(s * m * n);
     if (s == 1 || t < least) best = static_cast<int>(s), least = t;
   }
   return {0, 0, best};
@@ -761,12 +776,13 @@ void run_join(const float* partial, const void* bias, void* y, int64_t rows, int
                                                                                          relu);
 }
 
-constexpr int kThinLds = 64 * 1024;        // a workgroup's share: two on a CU
-int thin_waves(int panels) { return panels >= 16 ? 8 : (panels >= 4 ? 4 : 1); }
-// x is quantised inside the thin product: up to four rows, and up to 16 of 128 KB together, where they fit a workgroup's LDS in four bits. 8 rows of
-// 4096 float32: 10.3 against 12.9 us with a launch of its own; 16 rows of 2048: 12.7 against 12.6, the break-even; of 4096: 14.4 against 12.6.
+int thin_waves(int64_t panels) { return panels >= 16 ? 8 : (panels >= 4 ? 4 : 1); }
+// x is quantised inside the thin product where its values come in two rounds of loads or less - another round costs what the launch does that it saves
+// (float32, one round: a row of 4096 4.5 against 6.3 us; two: a row of 25088 15.5 against 17.6, 4 rows of 4096 6.8 against 7.0; three: 4 rows of 8192
+// 11.9 against 10.4)
 bool thin_raw(int64_t m, int64_t k, int bytes) {
-  return (m <= 4 || (m <= 16 && m * k * bytes <= 128 * 1024)) && panels_of(k) * m * 136 + 8 * 1024 <= kThinLds;
+  const int64_t panels = panels_of(k);
+  return m <= 16 && m * panels <= 2 * thin_waves(panels) * (bytes == 4 ? kThinBatch<4> : 2 * kThinBatch<8>);
 }
 
 template <class T, int MT, bool RAW>
@@ -781,8 +797,8 @@ int run_thin(Operand x, const void* values, int64_t k, Operand w, const void* bi
 template <class T, int BM, int BN>
 int run_tile(Operand x, Operand w, const void* bias, void* y, float* partial, int panels, int splits, int relu, hipStream_t st) {
   const int64_t tiles = ((x.rows + BM - 1) / BM) * ((w.rows + BN - 1) / BN) * splits;
-  if (!adv_internal_lds_limit<mx4_linear_tile<T, BM, BN>>(kTileLds<BM, BN>)) return ADV_ELAUNCH;
-  mx4_linear_tile<T, BM, BN><<<dim3(static_cast<unsigned>(tiles)), kBlock, kTileLds<BM, BN>, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), partial, panels,
+  if (!adv_internal_lds_limit<mx4_linear_tile<T, BM, BN>>(kTileStages<BM, BN> * kTileStage<BM, BN>)) return ADV_ELAUNCH;
+  mx4_linear_tile<T, BM, BN><<<dim3(static_cast<unsigned>(tiles)), kBlock, kTileStages<BM, BN> * kTileStage<BM, BN>, st>>>(x, w, static_cast<const T*>(bias), static_cast<T*>(y), partial, panels,
                                                                                                   splits, relu);
   if (splits > 1) run_join<T>(partial, bias, y, x.rows, w.rows, splits, relu, st);
   return adv_internal_finish_launch();
@@ -807,6 +823,8 @@ int run_linear(Operand x, const void* values, Operand w, const void* bias, void*
   float* partial = reinterpret_cast<float*>(ws + cb + sb);
   const int panels = static_cast<int>(panels_of(k));
   if (p.big) return run_tile<T, 256, 256>(x, w, bias, y, partial, panels, p.splits, relu, st);
+  if (x.rows <= 32) return run_tile<T, 32, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
+  if (x.rows <= 64) return run_tile<T, 64, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
   return run_tile<T, 128, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
 }
 

@@ -199,7 +199,8 @@ def close_product(got, a, b, dtype, bias, relu, per_step, what):
 
 
 LINEAR = [(1, 1, 1), (1, 32, 64), (2, 33, 31), (1, 4096, 2048), (16, 100, 257), (17, 31, 1000), (33, 65, 512), (64, 300, 25088), (65, 257, 1999), (130, 129, 4100),
-          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96), (2050, 4100, 300), (2047, 4090, 2100), (8, 40, 4096), (9, 70, 4097), (16, 50, 2048), (16, 90, 4000), (5, 1000, 6500), (13, 20, 16)]
+          (301, 2048, 700), (300, 40, 5000), (513, 520, 1024), (1030, 260, 96), (2050, 4100, 300), (2047, 4090, 2100), (8, 40, 4096), (9, 70, 4097), (16, 50, 2048), (16, 90, 4000), (5, 1000, 6500), (13, 20, 16),
+          (20, 140, 9000), (32, 129, 12544), (3, 200, 20000), (1, 50, 29000), (47, 300, 4400), (1, 40, 28672), (16, 33, 14400), (60, 4100, 1100)]
 
 
 @pytest.mark.gpu
