@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kBlock, BM < 128 ? 2 : 1) void mx4_linear_tile(Oper
   }
 }
 
-// y = relu?(part 0 + part 1 + ... + bias), in that order; four elements a thread.  14 parts of 32 x 4096: 6 us, latency (7 MB, from the caches)
+// y = relu?(part 0 + part 1 + ... + bias), in that order; four elements a thread.  Five parts of 301 x 2048: 5 us, latency (12 MB, from the caches)
 template <class T>
 __global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ partial, const T* __restrict__ bias, T* __restrict__ y, int64_t n, int64_t cols,
                                                    int parts, int relu) {
