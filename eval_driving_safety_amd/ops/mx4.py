@@ -37,7 +37,7 @@ class Mx4:
 
 
 def _made(codes, scales, shape, rows, cols):
-    """an Mx4 of tensors that were laid out here: the constructor's checks are a fifth of a small quantisation's call"""
+    """an Mx4 of tensors that were laid out here: the constructor's checks are an eighth of a small quantisation's call"""
     q = Mx4.__new__(Mx4)
     q.codes, q.scales, q.shape, q.rows, q.cols = codes, scales, shape, rows, cols
     return q
