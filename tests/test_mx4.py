@@ -324,8 +324,8 @@ def test_hip_graph_replays_and_streams():
     """two graphs that share nothing but the weights, replayed in turn with eager calls between, and a side stream"""
     from eval_driving_safety_amd import ops
     w, b = ops.mx4_quantize(make((300, 5000), torch.float32, 1)), make((300,), torch.float32, 2)
-    xs = [make((r, 5000), torch.float32, 3 + r) for r in (1, 37, 200)]
-    gs = [make((r, 300), torch.float32, 9 + r) for r in (1, 37, 200)]
+    xs = [make((r, 5000), torch.float32, 3 + r) for r in (1, 37, 60, 200)]
+    gs = [make((r, 300), torch.float32, 9 + r) for r in (1, 37, 60, 200)]
     static = [(x.clone(), g.clone()) for x, g in zip(xs, gs)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
