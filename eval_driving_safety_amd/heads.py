@@ -17,7 +17,9 @@ def layer_seed(seed, index):
 class LinearDropout(nn.Linear):
     """``relu?(dropout(linear(x)))`` with ``nn.Linear``'s parameters and state-dict keys.  In training every forward takes the next ``step`` (a plain
     number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device.  For a step captured in a
-    hipGraph set ``step`` to an int64 CUDA tensor of one element and move it on between the replays (a number would repeat one mask: refused)."""
+    hipGraph set ``step`` to an int64 CUDA tensor of one element and move it on between the replays (a number would repeat one mask: refused).  The same
+    where activations are recomputed in the backward pass (torch.utils.checkpoint): the second forward must draw the first one's mask, so ``step`` has to
+    be a tensor that is moved on after the backward pass (a number has moved on by then: refused)."""
 
     def __init__(self, linear, p, seed, relu=False):
         nn.Module.__init__(self)
@@ -34,6 +36,8 @@ class LinearDropout(nn.Linear):
         if not isinstance(step, torch.Tensor):
             if x.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("LinearDropout: a captured step needs `step` as an int64 CUDA tensor (a number would give every replay the same mask)")
+            if torch._C._current_graph_task_id() != -1:            # inside a backward pass
+                raise RuntimeError("LinearDropout: a forward recomputed in the backward pass needs `step` as an int64 tensor (the number has moved on: another mask)")
             self.step = step + 1
         y = F.linear(x, self.weight).contiguous()
         bias = self.bias if self.bias is None or self.bias.dtype == y.dtype else self.bias.to(y.dtype)      # (under autocast the product's type)

@@ -1,0 +1,76 @@
+"""The fully connected heads' layers (heads.py) in the hands of a program that does more than call them once: recomputed activations, a second seed, a
+head that was trained before it is quantised, checkpoints, hooks, a first call on a side stream.  Without a GPU the oracle stands in the kernel's place."""
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+from torch.utils.checkpoint import checkpoint
+
+from eval_driving_safety_amd import heads
+from oracle import oracle_np as O
+
+
+class OracleDropout(torch.autograd.Function):
+    """``ops.Dropout`` on the CPU, from the oracle"""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, step=0, bias=None, relu=False):
+        y = torch.tensor(O.dropout(x.detach().double().numpy(), p, seed, int(step), None if bias is None else bias.detach().double().numpy(), relu)).to(x.dtype)
+        ctx.save_for_backward(y if relu else None, step if isinstance(step, torch.Tensor) else None)
+        ctx.p, ctx.seed, ctx.step = p, seed, int(step)
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        y, step = ctx.saved_tensors
+        gx, gb = O.dropout_bwd(g.double().numpy(), ctx.p, ctx.seed, ctx.step if step is None else int(step), None if y is None else y.double().numpy())
+        return torch.tensor(gx).to(g.dtype), None, None, None, torch.tensor(gb).to(g.dtype) if ctx.needs_input_grad[4] else None, None
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    from eval_driving_safety_amd import ops
+    monkeypatch.setattr(ops, "Dropout", OracleDropout)
+
+
+def small_head(seed=0, p=0.5):
+    torch.manual_seed(seed)
+    return nn.Sequential(nn.Linear(24, 40), nn.Dropout(p), nn.ReLU(), nn.Linear(40, 3), nn.Dropout(p))
+
+
+def rows(n, seed=1):
+    return torch.randn(n, 24, generator=torch.Generator().manual_seed(seed))
+
+
+# ---------------------------------------------------------------------------------------------------------------- recomputed activations
+def recomputed_gradient(device, use_reentrant, step):
+    """(output, gradient w.r.t. the input) of a LinearDropout, and of the same one under activation recomputation"""
+    out = []
+    for recompute in (False, True):
+        h = small_head().to(device)
+        heads.counter_dropout(h, 5)
+        layer = h[0].train()
+        layer.step = step if isinstance(step, int) else step.clone()
+        x = rows(6).to(device).requires_grad_()
+        y = checkpoint(layer, x, use_reentrant=use_reentrant) if recompute else layer(x)
+        y.sum().backward()
+        out.append((y.detach(), x.grad))
+    return out
+
+
+def check_recomputation(device):
+    for use_reentrant in (False, True):
+        with pytest.raises(RuntimeError, match="recompute"):
+            recomputed_gradient(device, use_reentrant, 3)
+        (y, g), (yr, gr) = recomputed_gradient(device, use_reentrant, torch.full((1,), 3, dtype=torch.int64, device=device))
+        assert torch.equal(y, yr) and torch.equal(g, gr) and g.abs().max() > 0
+
+
+def test_a_recomputed_forward_is_refused_or_draws_the_same_mask(on_the_cpu):
+    """a numbered step has moved on when the forward runs again inside the backward pass: another mask than the loss saw - refused; a step tensor holds"""
+    check_recomputation(torch.device("cpu"))
+
+
+@pytest.mark.gpu
+def test_hip_a_recomputed_forward_is_refused_or_draws_the_same_mask():
+    check_recomputation(torch.device("cuda"))
