@@ -4,9 +4,13 @@
 the product is torch's, bias + dropout + ReLU are one kernel (``ops.Dropout``), and the mask of step s under a seed is the same in every process.
 ``Mx4LinearLayer`` stands for a frozen Linear (- ReLU) whose weight is held in MXFP4 (``ops.Mx4Linear``): gradients flow to its input only, as
 through every adopted layer."""
+import threading
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+_FIRST_USE = threading.Lock()
 
 
 def layer_seed(seed, index):
@@ -63,13 +67,28 @@ class Mx4LinearLayer(nn.Module):
         """the weight as ``ops.Mx4``"""
         from . import ops
         if self.codes is None:
-            if not self.weight.is_cuda:
+            self._quantise(ops)
+        return ops.Mx4(self.codes, self.scales, (self.out_features, self.in_features))
+
+    def _quantise(self, ops):
+        """First use, which may be on any stream and in any thread: on the device's default stream, behind what the caller's has been given (so that the
+        four bits belong where a module's tensors do), and finished before another stream sees them or the float weight is given up"""
+        with _FIRST_USE:
+            if self.codes is not None:           # another thread came first
+                return
+            weight = self.weight
+            if not weight.is_cuda:
                 raise RuntimeError("Mx4LinearLayer: libadvengine has no CPU path - move the model and its inputs to the ROCm device")
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("Mx4LinearLayer: run the layer once before capturing it (its weight is quantised on first use)")
-            q = ops.mx4_quantize(self.weight.contiguous())
-            self.codes, self.scales, self.weight = q.codes, q.scales, None
-        return ops.Mx4(self.codes, self.scales, (self.out_features, self.in_features))
+            home = torch.cuda.default_stream(weight.device)
+            home.wait_stream(torch.cuda.current_stream(weight.device))
+            with torch.inference_mode(False), torch.no_grad(), torch.cuda.stream(home):
+                q = ops.mx4_quantize(weight.contiguous())
+            home.synchronize()
+            self.scales = q.scales
+            self.codes = q.codes                 # (the one that held() asks for: last but the weight)
+            self.weight = None
 
     def forward(self, x):
         w = self.held()

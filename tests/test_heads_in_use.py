@@ -74,3 +74,56 @@ def test_a_recomputed_forward_is_refused_or_draws_the_same_mask(on_the_cpu):
 @pytest.mark.gpu
 def test_hip_a_recomputed_forward_is_refused_or_draws_the_same_mask():
     check_recomputation(torch.device("cuda"))
+
+
+# ---------------------------------------------------------------------------------------------------------------- first use
+@pytest.mark.gpu
+def test_hip_the_first_call_may_be_on_a_side_stream_and_the_second_on_another():
+    """the weight is quantised inside the first forward: a second stream's forward must find it finished, and memory handed out again on the stream that
+    made the float weight must not be read any more"""
+    import threading
+    from eval_driving_safety_amd import ops
+    torch.manual_seed(2)
+    lin = nn.Linear(4096, 2048).cuda()
+    x = torch.randn(9, 4096, generator=torch.Generator().manual_seed(2)).cuda()
+    want = ops.mx4_linear(x, ops.mx4_quantize(lin.weight.detach()), lin.bias.detach())
+    for threads in (False, True):
+        layer = nn.Sequential(heads.Mx4LinearLayer(lin))
+        torch.cuda.synchronize()
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        got = {}
+
+        def call(stream, name, wait):
+            with torch.no_grad(), torch.cuda.stream(stream):
+                if wait:
+                    torch.cuda._sleep(2_000_000)              # work in front of the first use
+                got[name] = layer(x)
+
+        if threads:
+            both = [threading.Thread(target=call, args=(s, n, True)) for s, n in ((a, "a"), (b, "b"))]
+            for t in both:
+                t.start()
+            for t in both:
+                t.join()
+        else:
+            call(a, "a", True)
+            spoil = [torch.full((2048, 4096), float("nan"), device="cuda") for _ in range(3)]      # the size of what the layer gave up
+            call(b, "b", False)
+            del spoil
+        torch.cuda.synchronize()
+        assert torch.equal(got["a"], want) and torch.equal(got["b"], want) and layer[0].weight is None
+
+
+@pytest.mark.gpu
+def test_hip_a_layer_first_run_in_inference_mode_carries_gradients_afterwards():
+    from eval_driving_safety_amd import ops
+    torch.manual_seed(3)
+    lin = nn.Linear(24, 8).cuda()
+    layer = heads.Mx4LinearLayer(lin)
+    x = rows(5).cuda()
+    with torch.inference_mode():
+        y = layer(x)
+    xr = x.clone().requires_grad_()
+    z = layer(xr)
+    z.sum().backward()
+    assert torch.equal(y, z) and torch.equal(xr.grad, ops.mx4_linear_dgrad(torch.ones_like(z), layer.held()))
