@@ -18,7 +18,22 @@ def layer_seed(seed, index):
     return (int(seed) + index * 0x9E3779B97F4A7C15) % (1 << 64)
 
 
-class LinearDropout(nn.Linear):
+class _Counted:
+    """dropout under ``seed`` whose every forward takes the next ``step``"""
+
+    def _drop(self, y, bias=None, relu=False):
+        from . import ops
+        step = self.step
+        if not isinstance(step, torch.Tensor):
+            if y.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("%s: a captured step needs `step` as an int64 CUDA tensor (a number would give every replay the same mask)" % type(self).__name__)
+            if torch._C._current_graph_task_id() != -1:            # inside a backward pass
+                raise RuntimeError("%s: a forward recomputed in the backward pass needs `step` as an int64 tensor (the number has moved on: another mask)" % type(self).__name__)
+            self.step = step + 1
+        return ops.Dropout.apply(y, self.p, self.seed, step, bias, relu)
+
+
+class LinearDropout(_Counted, nn.Linear):
     """``relu?(dropout(linear(x)))`` with ``nn.Linear``'s parameters and state-dict keys.  In training every forward takes the next ``step`` (a plain
     number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device.  For a step captured in a
     hipGraph set ``step`` to an int64 CUDA tensor of one element and move it on between the replays (a number would repeat one mask: refused).  The same
@@ -35,29 +50,23 @@ class LinearDropout(nn.Linear):
         if not self.training:
             y = F.linear(x, self.weight, self.bias)
             return F.relu(y) if self.relu else y
-        from . import ops
-        step = self.step
-        if not isinstance(step, torch.Tensor):
-            if x.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("LinearDropout: a captured step needs `step` as an int64 CUDA tensor (a number would give every replay the same mask)")
-            if torch._C._current_graph_task_id() != -1:            # inside a backward pass
-                raise RuntimeError("LinearDropout: a forward recomputed in the backward pass needs `step` as an int64 tensor (the number has moved on: another mask)")
-            self.step = step + 1
         y = F.linear(x, self.weight).contiguous()
         bias = self.bias if self.bias is None or self.bias.dtype == y.dtype else self.bias.to(y.dtype)      # (under autocast the product's type)
-        return ops.Dropout.apply(y, self.p, self.seed, step, bias, self.relu)
+        return self._drop(y, bias, self.relu)
 
     def extra_repr(self):
         return "%s, p=%g, seed=%d, relu=%s" % (nn.Linear.extra_repr(self), self.p, self.seed, self.relu)
 
 
-class Mx4LinearLayer(nn.Module):
+class Mx4LinearLayer(_Counted, nn.Module):
     """``relu?(linear(x))`` with the weight in MXFP4 and x quantised on the way in; the weight is quantised when the layer first runs on a ROCm device
-    (its float copy is given up then: code that reads the layer's ``weight`` does not work on it)"""
+    (its float copy is given up then: code that reads the layer's ``weight`` does not work on it).  Of a ``LinearDropout`` it keeps the dropout, rate, seed
+    and step: in training its output is dropped as before."""
 
     def __init__(self, linear, relu=False):
         super().__init__()
         self.in_features, self.out_features, self.relu = linear.in_features, linear.out_features, bool(relu)
+        self.p, self.seed, self.step = (linear.p, linear.seed, linear.step) if isinstance(linear, LinearDropout) else (0.0, 0, 0)
         self.register_buffer("weight", linear.weight.detach().clone())
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
         self.register_buffer("codes", None)
@@ -94,10 +103,11 @@ class Mx4LinearLayer(nn.Module):
         w = self.held()
         from . import ops
         bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
-        return ops.Mx4Linear.apply(x.contiguous(), w, bias, self.relu)
+        y = ops.Mx4Linear.apply(x.contiguous(), w, bias, self.relu)
+        return self._drop(y) if self.training and self.p else y        # (behind the ReLU as in front of it: the same values)
 
     def extra_repr(self):
-        return "%d -> %d, mxfp4%s" % (self.in_features, self.out_features, ", relu" if self.relu else "")
+        return "%d -> %d, mxfp4%s%s" % (self.in_features, self.out_features, ", relu" if self.relu else "", ", p=%g, seed=%d" % (self.p, self.seed) if self.p else "")
 
 
 def _is_relu(m):
@@ -124,22 +134,23 @@ def counter_dropout(module, seed):
 
 
 def mx4_linears(module, prefix=""):
-    """Replace, IN PLACE, every ``nn.Linear`` under ``module`` by ``Mx4LinearLayer`` (a ReLU that follows it in an ``nn.Sequential``, a Dropout between them
-    allowed, runs in its kernel: a dropped or scaled value keeps its sign).  -> [(qualified name, what)]"""
+    """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (a ReLU that follows it in an ``nn.Sequential``, a
+    Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  -> [(qualified name, what)]"""
     done = []
     for parent_name, parent in list(module.named_modules()):
         names = list(parent._modules)
         for i, name in enumerate(names):
             lin = parent._modules[name]
-            if type(lin) is not nn.Linear:
+            if type(lin) not in (nn.Linear, LinearDropout):
                 continue
             at = i + 1
             if isinstance(parent, nn.Sequential):
                 while at < len(names) and type(parent._modules[names[at]]) in (nn.Dropout, nn.Identity):
                     at += 1
-            relu = isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
+            follows = isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
+            relu = follows or (type(lin) is LinearDropout and lin.relu)
             parent._modules[name] = Mx4LinearLayer(lin, relu).train(lin.training)
-            if relu:
+            if follows:
                 parent._modules[names[at]] = nn.Identity().train(lin.training)
             done.append((prefix + (parent_name + "." if parent_name else "") + name, "linear %d->%d mxfp4%s" % (lin.in_features, lin.out_features, " + relu" if relu else "")))
     return done

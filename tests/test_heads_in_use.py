@@ -127,3 +127,63 @@ def test_hip_a_layer_first_run_in_inference_mode_carries_gradients_afterwards():
     z = layer(xr)
     z.sum().backward()
     assert torch.equal(y, z) and torch.equal(xr.grad, ops.mx4_linear_dgrad(torch.ones_like(z), layer.held()))
+
+
+# ---------------------------------------------------------------------------------------------------------------- trained, then quantised
+def test_a_head_trained_under_counter_dropout_is_quantised(on_the_cpu):
+    h = small_head()
+    heads.counter_dropout(h, 5)
+    h.train()
+    h(rows(2))
+    counted = [m for m in h if isinstance(m, heads.LinearDropout)]
+    done = heads.mx4_linears(h)
+    assert [n for n, _ in done] == ["0", "3"] and [w for _, w in done] == ["linear 24->40 mxfp4 + relu", "linear 40->3 mxfp4"]
+    held = [m for m in h if isinstance(m, heads.Mx4LinearLayer)]
+    assert [(m.relu, m.p, m.seed, m.step, m.training) for m in held] == [(m.relu, m.p, m.seed, 1, True) for m in counted]
+    for m, c in zip(held, counted):
+        assert torch.equal(m.weight, c.weight) and torch.equal(m.bias, c.bias) and not m.weight.requires_grad
+
+
+def test_adopt_quantises_a_head_trained_under_counter_dropout():
+    from eval_driving_safety_amd import adopt as A
+    h = nn.Sequential(small_head())
+    heads.counter_dropout(h, 5)
+    report = A.adopt(h.eval(), linear="mxfp4", functional=False)
+    assert [n for n, _ in report["replaced"]] == ["0.0", "0.3"]
+
+
+@pytest.mark.gpu
+def test_hip_train_then_quantise_then_validate(tmp_path):
+    """classifiers.train under a dropout seed, quantize_head, check_accuracy: the accuracy is that of the four-bit layers; in training the dropout is the
+    one the layer had"""
+    from eval_driving_safety_amd import classifiers as C, ops
+
+    class Tiny(nn.Module):
+        head_key = "classifier"
+
+        def __init__(self):
+            super().__init__()
+            torch.manual_seed(4)
+            self.net = nn.Module()
+            self.net.classifier = nn.Sequential(nn.Linear(24, 40), nn.Dropout(0.1), nn.ReLU(), nn.Linear(40, 1), nn.Dropout(0.1), nn.Sigmoid())
+
+        backbone = property(lambda self: self.net)
+
+        def forward(self, x):
+            return self.net.classifier(x).squeeze(1)
+
+    data = [(rows(16, 7 + k), (rows(16, 7 + k)[:, 0] > 0).float()) for k in range(4)]
+    m = C.train("driving_constraint", data, None, torch.device("cuda"), str(tmp_path), epochs=2, model=Tiny(), log=lambda *a: None, dropout_seed=7)
+    head = m.net.classifier
+    (w1, b1), (w2, b2) = [(ops.mx4_quantize(q.weight.detach()), q.bias.detach()) for q in head if isinstance(q, heads.LinearDropout)]
+    assert [n for n, _ in C.quantize_head(m)] == ["classifier.0", "classifier.3"]
+    acc = C.check_accuracy(data, m, torch.device("cuda"), log=lambda *a: None)
+    right = sum(int(((torch.sigmoid(ops.mx4_linear(ops.mx4_linear(x.cuda(), w1, b1, True), w2, b2))[:, 0] >= 0.5) == (t.cuda() > 0)).sum()) for x, t in data)
+    assert acc == right / 64 * 100
+    layer, x = head[0], data[0][0].cuda()
+    assert layer.training and layer.p == 0.1 and layer.step == 8                  # as check_accuracy leaves the model; two epochs of four batches
+    plain = layer.eval()(x)
+    dropped = layer.train()(x)
+    kept = O.dropout_kept(0, 16 * 40, 0.1, layer.seed, 8).reshape(16, 40)
+    np.testing.assert_allclose(dropped.detach().cpu().numpy(), np.where(kept, plain.cpu().numpy() / 0.9, 0), rtol=3 * 2.0 ** -23, atol=0)
+    assert layer.step == 9
