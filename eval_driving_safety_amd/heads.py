@@ -116,16 +116,26 @@ def _is_relu(m):
 
 def counter_dropout(module, seed):
     """Replace, IN PLACE, every ``Linear, Dropout(, ReLU)`` run of consecutive children of an ``nn.Sequential`` in ``module`` by ``LinearDropout`` and
-    identities - the places in the sequence, hence the state-dict keys, stay.  -> the number of dropout layers replaced."""
+    identities - the places in the sequence, hence the state-dict keys, stay.  A ``LinearDropout`` that is there already goes over to ``seed``: from step 0,
+    or, where it has run under that seed before, on from its own step.  -> the number of dropout layers that now draw under ``seed``."""
     count = 0
-    for parent in [m for m in module.modules() if isinstance(m, nn.Sequential)]:
+    for parent in list(module.modules()):
         names = list(parent._modules)
-        for i in range(len(names) - 1):
-            lin, drop = parent._modules[names[i]], parent._modules[names[i + 1]]
+        for i, name in enumerate(names):
+            lin = parent._modules[name]
+            if type(lin) is LinearDropout:
+                own = layer_seed(seed, count)
+                if lin.seed != own:
+                    lin.seed = own
+                    if not isinstance(lin.step, torch.Tensor):           # (a step tensor is the program's to move)
+                        lin.step = 0
+                count += 1
+                continue
+            drop = parent._modules[names[i + 1]] if isinstance(parent, nn.Sequential) and i + 1 < len(names) else None
             if type(lin) is not nn.Linear or type(drop) is not nn.Dropout:
                 continue
             relu = i + 2 < len(names) and _is_relu(parent._modules[names[i + 2]])
-            parent._modules[names[i]] = LinearDropout(lin, drop.p, layer_seed(seed, count), relu).train(lin.training)
+            parent._modules[name] = LinearDropout(lin, drop.p, layer_seed(seed, count), relu).train(lin.training)
             parent._modules[names[i + 1]] = nn.Identity().train(lin.training)
             if relu:
                 parent._modules[names[i + 2]] = nn.Identity().train(lin.training)

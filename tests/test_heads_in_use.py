@@ -187,3 +187,18 @@ def test_hip_train_then_quantise_then_validate(tmp_path):
     kept = O.dropout_kept(0, 16 * 40, 0.1, layer.seed, 8).reshape(16, 40)
     np.testing.assert_allclose(dropped.detach().cpu().numpy(), np.where(kept, plain.cpu().numpy() / 0.9, 0), rtol=3 * 2.0 ** -23, atol=0)
     assert layer.step == 9
+
+
+# ---------------------------------------------------------------------------------------------------------------- another seed
+def test_a_second_seed_takes_the_place_of_the_first(on_the_cpu):
+    h, fresh = small_head(), small_head()
+    assert heads.counter_dropout(h, 7) == 2
+    h.train()
+    h(rows(2)), h(rows(2))
+    assert heads.counter_dropout(h, 8) == 2 and heads.counter_dropout(fresh, 8) == 2
+    layers, new = [[m for m in q if isinstance(m, heads.LinearDropout)] for q in (h, fresh)]
+    assert [(m.seed, m.step) for m in layers] == [(m.seed, 0) for m in new]
+    assert torch.equal(h(rows(4)), fresh.train()(rows(4)))                       # as a model that never had another
+    assert heads.counter_dropout(h, 8) == 2 and [m.step for m in layers] == [1, 1]        # the same seed again: its masks are not repeated
+    layers[0].step = torch.tensor([5])
+    assert heads.counter_dropout(nn.ModuleDict({"a": layers[0]}), 3) == 1 and int(layers[0].step) == 5 and layers[0].seed == heads.layer_seed(3, 0)
