@@ -259,6 +259,8 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
         raise ValueError("adopt() needs the model in eval mode (BatchNorm statistics are folded)")
     if linear not in (None, "mxfp4"):
         raise ValueError("linear must be None or 'mxfp4', got %r" % (linear,))
+    if linear is not None and isinstance(model, nn.Linear):
+        raise ValueError("adopt() replaces layers in the module that holds them: a %s by itself cannot be adopted" % type(model).__name__)
     before = rng = None
     if verify is not None:
         rng = _rng_snapshot()
@@ -314,6 +316,8 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
     for name, m in model.named_modules():
         if isinstance(m, (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.ConvTranspose2d, nn.ConvTranspose3d)):
             report["kept"].append((name, type(m).__name__ + ": no libadvengine counterpart for this module type here"))
+        elif linear is not None and isinstance(m, nn.Linear):
+            report["kept"].append((name, type(m).__name__ + ": a subclass of Linear, kept in float"))
         elif isinstance(m, (nn.BatchNorm2d, nn.BatchNorm3d)):
             report["kept"].append((name, "BatchNorm not next to a convolution by either convention: left as it is"))
     # the FPN top-down path of the reference's detector class: ``_upsample_add(x, y)`` = F.interpolate(x, size=y's, mode='bilinear',

@@ -158,10 +158,22 @@ def freeze_backbone(model, train_backbone=False):
 
 def quantize_head(model):
     """the head's Linear layers with their weights in MXFP4 (``heads.Mx4LinearLayer``), in place, for ``check_accuracy`` and for gradients w.r.t. the
-    images; the backbone stays as it is.  Needs a ROCm device when it runs.  -> [(qualified name, what)]"""
+    images; the backbone stays as it is.  Needs a ROCm device when it runs.  A head of which a layer would stay in float is refused; of one that is in
+    four bits already nothing is left to do.  -> [(qualified name, what)]"""
     from . import heads
     head = getattr(model.backbone, model.head_key)
-    return heads.mx4_linears(head, prefix=model.head_key + ".")
+    if type(head) in (nn.Linear, heads.LinearDropout):
+        whole = nn.ModuleDict({model.head_key: head})
+        done = heads.mx4_linears(whole)
+        setattr(model.backbone, model.head_key, whole[model.head_key])
+        return done
+    other = [(name, kind) for name, kind in heads.float_linears(head, model.head_key + ".") if kind not in ("Linear", "LinearDropout")]
+    if other:
+        raise ValueError("quantize_head: %s would stay in float" % ", ".join("%s (%s)" % q for q in other))
+    done = heads.mx4_linears(head, prefix=model.head_key + ".")
+    if not done and not any(isinstance(m, heads.Mx4LinearLayer) for m in head.modules()):
+        raise ValueError("quantize_head: the head (%s) has no Linear layer" % model.head_key)
+    return done
 
 
 # ------------------------------------------------------------------------------------------------ data
@@ -232,13 +244,14 @@ def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=N
     learning rate stays 1e-3 - kept.
 
     ``dropout_seed``: the head's Linear - Dropout - ReLU runs on ``ops.Dropout`` under this seed - the masks are a function of the seed and the step,
-    not of the process's generator (None: torch's dropout, as the scripts have it)."""
+    not of the process's generator (None: the model's own dropout, torch's unless it was replaced before).  A head without a Linear - Dropout is refused."""
     cls, lr, n_epochs, _, val_every, save_every, _ = TASKS[task]
     model = (cls() if model is None else model).to(device)
     freeze_backbone(model, train_backbone)
     if dropout_seed is not None:
         from . import heads
-        heads.counter_dropout(getattr(model.backbone, model.head_key), dropout_seed)
+        if not heads.counter_dropout(getattr(model.backbone, model.head_key), dropout_seed):
+            raise ValueError("dropout_seed: the head (%s) has no Linear, Dropout in a Sequential" % model.head_key)
     criterion = nn.BCELoss()
     optimizer = torch.optim.Adam(model.parameters(), lr=lr)
     os.makedirs(save_dir, exist_ok=True)

@@ -145,7 +145,10 @@ def counter_dropout(module, seed):
 
 def mx4_linears(module, prefix=""):
     """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (a ReLU that follows it in an ``nn.Sequential``, a
-    Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  -> [(qualified name, what)]"""
+    Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear`` stay (``float_linears``
+    names them).  -> [(qualified name, what)]"""
+    if type(module) in (nn.Linear, LinearDropout):
+        raise ValueError("mx4_linears: a layer cannot be replaced in place without the module that holds it: build a heads.Mx4LinearLayer of it")
     done = []
     for parent_name, parent in list(module.named_modules()):
         names = list(parent._modules)
@@ -164,3 +167,8 @@ def mx4_linears(module, prefix=""):
                 parent._modules[names[at]] = nn.Identity().train(lin.training)
             done.append((prefix + (parent_name + "." if parent_name else "") + name, "linear %d->%d mxfp4%s" % (lin.in_features, lin.out_features, " + relu" if relu else "")))
     return done
+
+
+def float_linears(module, prefix=""):
+    """[(qualified name, type's name)] of the layers under ``module`` (itself included) whose product is still ``nn.Linear``'s or a subclass's"""
+    return [(prefix + name, type(m).__name__) for name, m in module.named_modules() if isinstance(m, nn.Linear)]

@@ -202,3 +202,46 @@ def test_a_second_seed_takes_the_place_of_the_first(on_the_cpu):
     assert heads.counter_dropout(h, 8) == 2 and [m.step for m in layers] == [1, 1]        # the same seed again: its masks are not repeated
     layers[0].step = torch.tensor([5])
     assert heads.counter_dropout(nn.ModuleDict({"a": layers[0]}), 3) == 1 and int(layers[0].step) == 5 and layers[0].seed == heads.layer_seed(3, 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------- nothing to replace
+def holder(head):
+    class Model(nn.Module):
+        head_key = "fc"
+
+        def __init__(self):
+            super().__init__()
+            self.net = nn.Module()
+            self.net.fc = head
+
+        backbone = property(lambda self: self.net)
+
+        def forward(self, x):
+            return self.net.fc(x).squeeze(1)
+
+    return Model()
+
+
+class OwnLinear(nn.Linear):
+    pass
+
+
+def test_a_head_of_which_nothing_can_be_replaced_is_refused(tmp_path):
+    from eval_driving_safety_amd import adopt as A, classifiers as C
+    with pytest.raises(ValueError, match="no Linear layer"):
+        C.quantize_head(holder(nn.Sequential(nn.Sigmoid())))
+    with pytest.raises(ValueError, match="fc.1 .OwnLinear."):
+        C.quantize_head(holder(nn.Sequential(nn.Linear(4, 4), OwnLinear(4, 1))))
+    with pytest.raises(ValueError, match="cannot be replaced in place"):
+        heads.mx4_linears(nn.Linear(4, 4))
+    with pytest.raises(ValueError, match="cannot be adopted"):
+        A.adopt(nn.Linear(4, 4).eval(), linear="mxfp4", functional=False)
+    report = A.adopt(nn.Sequential(nn.Linear(4, 4), OwnLinear(4, 1)).eval(), linear="mxfp4", functional=False)
+    assert [n for n, _ in report["replaced"]] == ["0"] and [n for n, _ in report["kept"]] == ["1"]
+    m = holder(nn.Linear(4, 1))                                                   # a head that is one layer
+    assert C.quantize_head(m) == [("fc", "linear 4->1 mxfp4")] and isinstance(m.net.fc, heads.Mx4LinearLayer)
+    m = holder(nn.Sequential(nn.Linear(4, 1)))
+    assert len(C.quantize_head(m)) == 1 and C.quantize_head(m) == []              # nothing left to do
+    for head in (nn.Sequential(nn.Linear(4, 1), nn.Sigmoid()), nn.Linear(4, 1)):
+        with pytest.raises(ValueError, match="dropout_seed"):
+            C.train("driving_constraint", [], None, torch.device("cpu"), str(tmp_path), epochs=1, model=holder(head), log=lambda *a: None, dropout_seed=1)
