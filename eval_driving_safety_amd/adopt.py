@@ -312,7 +312,7 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
             report["replaced"].append((_q(parent_name, name), getattr(parent, name).kind))
     if linear is not None:
         from . import heads
-        report["replaced"] += heads.mx4_linears(model)
+        report["replaced"] += heads.mx4_linears(model, fuse_relu=fuse_relu)
     for name, m in model.named_modules():
         if isinstance(m, (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.ConvTranspose2d, nn.ConvTranspose3d)):
             report["kept"].append((name, type(m).__name__ + ": no libadvengine counterpart for this module type here"))

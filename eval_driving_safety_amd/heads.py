@@ -143,9 +143,9 @@ def counter_dropout(module, seed):
     return count
 
 
-def mx4_linears(module, prefix=""):
-    """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (a ReLU that follows it in an ``nn.Sequential``, a
-    Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear`` stay (``float_linears``
+def mx4_linears(module, prefix="", fuse_relu=True):
+    """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (``fuse_relu``: a ReLU that follows it in an
+    ``nn.Sequential``, a Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear`` stay (``float_linears``
     names them).  -> [(qualified name, what)]"""
     if type(module) in (nn.Linear, LinearDropout):
         raise ValueError("mx4_linears: a layer cannot be replaced in place without the module that holds it: build a heads.Mx4LinearLayer of it")
@@ -160,7 +160,7 @@ def mx4_linears(module, prefix=""):
             if isinstance(parent, nn.Sequential):
                 while at < len(names) and type(parent._modules[names[at]]) in (nn.Dropout, nn.Identity):
                     at += 1
-            follows = isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
+            follows = fuse_relu and isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
             relu = follows or (type(lin) is LinearDropout and lin.relu)
             parent._modules[name] = Mx4LinearLayer(lin, relu).train(lin.training)
             if follows:

@@ -245,3 +245,11 @@ def test_a_head_of_which_nothing_can_be_replaced_is_refused(tmp_path):
     for head in (nn.Sequential(nn.Linear(4, 1), nn.Sigmoid()), nn.Linear(4, 1)):
         with pytest.raises(ValueError, match="dropout_seed"):
             C.train("driving_constraint", [], None, torch.device("cpu"), str(tmp_path), epochs=1, model=holder(head), log=lambda *a: None, dropout_seed=1)
+
+
+def test_adopt_leaves_relus_alone_where_it_is_told_to():
+    from eval_driving_safety_amd import adopt as A
+    for fuse in (True, False):
+        h = small_head().eval()
+        A.adopt(h, fuse_relu=fuse, linear="mxfp4", functional=False)
+        assert h[0].relu is fuse and isinstance(h[2], nn.Identity if fuse else nn.ReLU)
