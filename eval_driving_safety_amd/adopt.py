@@ -261,6 +261,9 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
         raise ValueError("linear must be None or 'mxfp4', got %r" % (linear,))
     if linear is not None and isinstance(model, nn.Linear):
         raise ValueError("adopt() replaces layers in the module that holds them: a %s by itself cannot be adopted" % type(model).__name__)
+    if linear is not None:
+        from . import heads
+        heads.refuse_hooked_linears(model)            # (before anything is replaced)
     before = rng = None
     if verify is not None:
         rng = _rng_snapshot()
@@ -311,7 +314,6 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
                 report["folded_bn"] += 1
             report["replaced"].append((_q(parent_name, name), getattr(parent, name).kind))
     if linear is not None:
-        from . import heads
         report["replaced"] += heads.mx4_linears(model, fuse_relu=fuse_relu)
     for name, m in model.named_modules():
         if isinstance(m, (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.ConvTranspose2d, nn.ConvTranspose3d)):

@@ -111,13 +111,31 @@ class Mx4LinearLayer(_Counted, nn.Module):
 
 
 def _is_relu(m):
-    return isinstance(m, nn.ReLU) or type(m).__name__ == "_ReLU"
+    """a ReLU that a layer in front of it may take over (one with hooks keeps its place: they want its own result)"""
+    return (isinstance(m, nn.ReLU) or type(m).__name__ == "_ReLU") and not _hooked(m)
+
+
+def _hooked(m):
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def _refuse_hooks(who, name, m):
+    """Hooks see a layer's own input and result, or make its weight (torch.nn.utils.weight_norm: trained through two other parameters): neither goes over
+    to what takes the layer's place"""
+    if _hooked(m):
+        raise ValueError("%s: %s (%s) has hooks, which its replacement would not run: remove them first" % (who, name, type(m).__name__))
 
 
 def counter_dropout(module, seed):
     """Replace, IN PLACE, every ``Linear, Dropout(, ReLU)`` run of consecutive children of an ``nn.Sequential`` in ``module`` by ``LinearDropout`` and
     identities - the places in the sequence, hence the state-dict keys, stay.  A ``LinearDropout`` that is there already goes over to ``seed``: from step 0,
     or, where it has run under that seed before, on from its own step.  -> the number of dropout layers that now draw under ``seed``."""
+    for parent_name, parent in module.named_modules():                   # (before anything is replaced)
+        children = list(parent._modules.items())
+        for (name, lin), (drop_name, drop) in zip(children, children[1:]):
+            if isinstance(parent, nn.Sequential) and type(lin) is nn.Linear and type(drop) is nn.Dropout:
+                _refuse_hooks("counter_dropout", (parent_name + "." if parent_name else "") + name, lin)
+                _refuse_hooks("counter_dropout", (parent_name + "." if parent_name else "") + drop_name, drop)
     count = 0
     for parent in list(module.modules()):
         names = list(parent._modules)
@@ -149,6 +167,7 @@ def mx4_linears(module, prefix="", fuse_relu=True):
     names them).  -> [(qualified name, what)]"""
     if type(module) in (nn.Linear, LinearDropout):
         raise ValueError("mx4_linears: a layer cannot be replaced in place without the module that holds it: build a heads.Mx4LinearLayer of it")
+    refuse_hooked_linears(module, prefix)
     done = []
     for parent_name, parent in list(module.named_modules()):
         names = list(parent._modules)
@@ -158,7 +177,7 @@ def mx4_linears(module, prefix="", fuse_relu=True):
                 continue
             at = i + 1
             if isinstance(parent, nn.Sequential):
-                while at < len(names) and type(parent._modules[names[at]]) in (nn.Dropout, nn.Identity):
+                while at < len(names) and type(parent._modules[names[at]]) in (nn.Dropout, nn.Identity) and not _hooked(parent._modules[names[at]]):
                     at += 1
             follows = fuse_relu and isinstance(parent, nn.Sequential) and at < len(names) and _is_relu(parent._modules[names[at]])
             relu = follows or (type(lin) is LinearDropout and lin.relu)
@@ -167,6 +186,13 @@ def mx4_linears(module, prefix="", fuse_relu=True):
                 parent._modules[names[at]] = nn.Identity().train(lin.training)
             done.append((prefix + (parent_name + "." if parent_name else "") + name, "linear %d->%d mxfp4%s" % (lin.in_features, lin.out_features, " + relu" if relu else "")))
     return done
+
+
+def refuse_hooked_linears(module, prefix=""):
+    """raises if a layer that ``mx4_linears`` would replace has hooks"""
+    for name, m in module.named_modules():
+        if type(m) in (nn.Linear, LinearDropout):
+            _refuse_hooks("mx4_linears", prefix + name, m)
 
 
 def float_linears(module, prefix=""):

@@ -253,3 +253,35 @@ def test_adopt_leaves_relus_alone_where_it_is_told_to():
         h = small_head().eval()
         A.adopt(h, fuse_relu=fuse, linear="mxfp4", functional=False)
         assert h[0].relu is fuse and isinstance(h[2], nn.Identity if fuse else nn.ReLU)
+
+
+# ---------------------------------------------------------------------------------------------------------------- hooks
+def test_hooked_layers_are_refused_and_hooked_relus_keep_their_place():
+    import warnings
+    from eval_driving_safety_amd import adopt as A
+    hooks = (lambda m: m.register_forward_hook(lambda *a: None), lambda m: m.register_forward_pre_hook(lambda *a: None),
+             lambda m: m.register_full_backward_hook(lambda *a: None), lambda m: m.register_full_backward_pre_hook(lambda *a: None))
+    for add in hooks:
+        for replace in (lambda q: heads.counter_dropout(q, 1), heads.mx4_linears, lambda q: A.adopt(q.eval(), linear="mxfp4", functional=False)):
+            h = nn.Sequential(nn.Conv2d(1, 1, 1), nn.ReLU(), small_head())
+            add(h[2][3])
+            kinds = [type(m) for m in h.modules()]
+            with pytest.raises(ValueError, match="2.3 .Linear. has hooks"):
+                replace(h)
+            assert [type(m) for m in h.modules()] == kinds                          # nothing was replaced
+        h = small_head()
+        add(h[1])
+        with pytest.raises(ValueError, match="1 .Dropout. has hooks"):
+            heads.counter_dropout(h, 1)
+        heads.mx4_linears(h)
+        assert not h[0].relu and isinstance(h[2], nn.ReLU)                          # its hook sees what it saw
+        for replace in (lambda q: heads.counter_dropout(q, 1), heads.mx4_linears):
+            h = small_head()
+            add(h[2])
+            replace(h)
+            assert not h[0].relu and isinstance(h[2], nn.ReLU)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        h = nn.Sequential(nn.utils.weight_norm(nn.Linear(4, 4)), nn.Dropout(0.1))      # its weight is made by a hook, of two other parameters
+    with pytest.raises(ValueError, match="hooks"):
+        heads.counter_dropout(h, 1)
