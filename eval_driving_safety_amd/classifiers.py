@@ -244,14 +244,19 @@ def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=N
     learning rate stays 1e-3 - kept.
 
     ``dropout_seed``: the head's Linear - Dropout - ReLU runs on ``ops.Dropout`` under this seed - the masks are a function of the seed and the step,
-    not of the process's generator (None: the model's own dropout, torch's unless it was replaced before).  A head without a Linear - Dropout is refused."""
+    not of the process's generator (None: the model's own dropout, torch's unless it was replaced before).  A head without a Linear - Dropout, or
+    with a dropout elsewhere, is refused."""
     cls, lr, n_epochs, _, val_every, save_every, _ = TASKS[task]
     model = (cls() if model is None else model).to(device)
     freeze_backbone(model, train_backbone)
     if dropout_seed is not None:
         from . import heads
-        if not heads.counter_dropout(getattr(model.backbone, model.head_key), dropout_seed):
+        head = getattr(model.backbone, model.head_key)
+        if not heads.counter_dropout(head, dropout_seed):
             raise ValueError("dropout_seed: the head (%s) has no Linear, Dropout in a Sequential" % model.head_key)
+        left = [name for name, m in head.named_modules() if isinstance(m, nn.modules.dropout._DropoutNd) and m.p > 0]
+        if left:
+            raise ValueError("dropout_seed: %s.%s does not follow a Linear: its mask would still come from the process's generator" % (model.head_key, left[0]))
     criterion = nn.BCELoss()
     optimizer = torch.optim.Adam(model.parameters(), lr=lr)
     os.makedirs(save_dir, exist_ok=True)

@@ -285,3 +285,10 @@ def test_hooked_layers_are_refused_and_hooked_relus_keep_their_place():
         h = nn.Sequential(nn.utils.weight_norm(nn.Linear(4, 4)), nn.Dropout(0.1))      # its weight is made by a hook, of two other parameters
     with pytest.raises(ValueError, match="hooks"):
         heads.counter_dropout(h, 1)
+
+
+def test_a_dropout_that_would_still_draw_from_the_process_is_refused(tmp_path):
+    from eval_driving_safety_amd import classifiers as C
+    head = nn.Sequential(nn.Linear(4, 4), nn.Dropout(0.1), nn.Linear(4, 4), nn.ReLU(), nn.Dropout(0.2), nn.Linear(4, 1))
+    with pytest.raises(ValueError, match="fc.4 does not follow a Linear"):
+        C.train("driving_constraint", [], None, torch.device("cpu"), str(tmp_path), epochs=1, model=holder(head), log=lambda *a: None, dropout_seed=1)
