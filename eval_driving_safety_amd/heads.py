@@ -61,7 +61,8 @@ class LinearDropout(_Counted, nn.Linear):
 class Mx4LinearLayer(_Counted, nn.Module):
     """``relu?(linear(x))`` with the weight in MXFP4 and x quantised on the way in; the weight is quantised when the layer first runs on a ROCm device
     (its float copy is given up then: code that reads the layer's ``weight`` does not work on it).  Of a ``LinearDropout`` it keeps the dropout, rate, seed
-    and step: in training its output is dropped as before."""
+    and step: in training its output is dropped as before.  A state dict holds the float weight or, of a layer that has run, its four bits; a layer in either
+    form takes either."""
 
     def __init__(self, linear, relu=False):
         super().__init__()
@@ -98,6 +99,24 @@ class Mx4LinearLayer(_Counted, nn.Module):
             self.scales = q.scales
             self.codes = q.codes                 # (the one that held() asks for: last but the weight)
             self.weight = None
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        weight, codes, scales = [state_dict.get(prefix + k) for k in ("weight", "codes", "scales")]
+        if codes is not None and scales is not None and weight is None and self.codes is None:
+            shape = ((self.in_features + 255) // 256, self.out_features)
+            self.codes, self.scales = [torch.empty(shape + (n,), dtype=torch.uint8, device=self.weight.device) for n in (128, 8)]
+            self.weight = None
+        elif weight is not None and codes is None and scales is None and self.codes is not None:
+            if not self.codes.is_cuda:                                       # (moved to the CPU, where nothing is quantised: as it was before it ran)
+                self.weight = torch.empty((self.out_features, self.in_features), dtype=weight.dtype, device=self.codes.device)
+                self.codes = self.scales = None
+            elif tuple(weight.shape) == (self.out_features, self.in_features):
+                from . import ops
+                held = weight.detach().to(self.codes.device, weight.dtype if weight.dtype in ops._FLOATS else torch.float32)
+                q = ops.mx4_quantize(held.contiguous())                      # into the tensors that are there: a captured graph reads those
+                state_dict = {k: v for k, v in state_dict.items() if k != prefix + "weight"}
+                state_dict[prefix + "codes"], state_dict[prefix + "scales"] = q.codes, q.scales
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def forward(self, x):
         w = self.held()

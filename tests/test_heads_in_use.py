@@ -292,3 +292,68 @@ def test_a_dropout_that_would_still_draw_from_the_process_is_refused(tmp_path):
     head = nn.Sequential(nn.Linear(4, 4), nn.Dropout(0.1), nn.Linear(4, 4), nn.ReLU(), nn.Dropout(0.2), nn.Linear(4, 1))
     with pytest.raises(ValueError, match="fc.4 does not follow a Linear"):
         C.train("driving_constraint", [], None, torch.device("cpu"), str(tmp_path), epochs=1, model=holder(head), log=lambda *a: None, dropout_seed=1)
+
+
+# ---------------------------------------------------------------------------------------------------------------- state dicts
+def four_bit_layer(lin, codes):
+    """a Mx4LinearLayer as it is after its first run"""
+    layer = heads.Mx4LinearLayer(lin)
+    layer.codes, layer.scales, layer.weight = torch.randint(0, 256, codes, dtype=torch.uint8), torch.randint(100, 150, codes[:2] + (8,), dtype=torch.uint8), None
+    return layer
+
+
+def test_a_layer_in_either_form_takes_either_state():
+    used, lin = four_bit_layer(nn.Linear(300, 5), (2, 5, 128)), nn.Linear(300, 5)
+    fresh = heads.Mx4LinearLayer(nn.Linear(300, 5))
+    fresh.load_state_dict(used.state_dict())
+    assert fresh.weight is None and torch.equal(fresh.codes, used.codes) and torch.equal(fresh.scales, used.scales) and torch.equal(fresh.bias, used.bias)
+    again = four_bit_layer(nn.Linear(300, 5), (2, 5, 128))
+    again.load_state_dict(used.state_dict())
+    assert torch.equal(again.codes, used.codes)
+    for strict in (True, False):
+        used.load_state_dict(lin.state_dict(), strict=strict)                       # on the CPU: float until it runs on a device
+        assert used.codes is None and used.scales is None and torch.equal(used.weight, lin.weight) and torch.equal(used.bias, lin.bias)
+        used = four_bit_layer(nn.Linear(300, 5), (2, 5, 128))
+    net, state = nn.Sequential(nn.ReLU(), heads.Mx4LinearLayer(nn.Linear(300, 5))), nn.Sequential(nn.ReLU(), used).state_dict()
+    net.load_state_dict(state)
+    assert torch.equal(net[1].codes, used.codes)
+    for bad in (nn.Linear(299, 5), nn.Linear(300, 6)):
+        for layer in (used, heads.Mx4LinearLayer(lin)):
+            with pytest.raises(RuntimeError):
+                layer.load_state_dict(bad.state_dict())
+            used = four_bit_layer(nn.Linear(300, 5), (2, 5, 128))
+    with pytest.raises(RuntimeError):
+        heads.Mx4LinearLayer(nn.Linear(256, 5)).load_state_dict(used.state_dict())
+    with pytest.raises(RuntimeError):
+        heads.Mx4LinearLayer(lin).load_state_dict({k: v for k, v in used.state_dict().items() if k != "scales"})
+
+
+@pytest.mark.gpu
+def test_hip_float_weights_loaded_into_a_layer_that_has_run():
+    """they are quantised into the tensors that are there: the eager call and a graph that was captured before give the new layer's values"""
+    from eval_driving_safety_amd import ops
+    torch.manual_seed(6)
+    a, b = nn.Linear(300, 70).cuda(), nn.Linear(300, 70).cuda()
+    x = torch.randn(40, 300, generator=torch.Generator().manual_seed(6)).cuda()
+    want = [ops.mx4_linear(x, ops.mx4_quantize(q.weight.detach()), q.bias.detach()) for q in (a, b)]
+    layer = heads.Mx4LinearLayer(a)
+    with torch.no_grad():
+        assert torch.equal(layer(x), want[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(x)
+        for lin, w in ((b, want[1]), (a, want[0]), (b, want[1])):
+            for strict, move in ((True, "cuda"), (False, "cpu")):
+                layer.load_state_dict({k: v.to(move) for k, v in lin.state_dict().items()}, strict=strict)
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(layer(x), w) and torch.equal(y, w) and layer.weight is None
+        fresh = heads.Mx4LinearLayer(a).cuda()
+        fresh.load_state_dict(layer.state_dict())
+        assert torch.equal(fresh(x), want[1])
+        layer.load_state_dict({"weight": b.weight.double(), "bias": b.bias})
+        assert torch.equal(layer(x), want[1])
+        with pytest.raises(RuntimeError):
+            layer.load_state_dict(nn.Linear(299, 70).state_dict())
+        # (as any module's: of a state that does not fit, the tensors that do - the bias - are taken before the error)
+        assert torch.equal(layer(x), ops.mx4_linear(x, ops.mx4_quantize(b.weight.detach()), layer.bias))
