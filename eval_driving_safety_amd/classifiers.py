@@ -245,12 +245,13 @@ def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=N
 
     ``dropout_seed``: the head's Linear - Dropout - ReLU runs on ``ops.Dropout`` under this seed - the masks are a function of the seed and the step,
     not of the process's generator (None: the model's own dropout, torch's unless it was replaced before).  A head without a Linear - Dropout, or
-    with a dropout elsewhere, is refused."""
+    with a dropout elsewhere, is refused.  The checkpoints then hold seed and step of each layer; to go on from one: ``heads.counter_dropout`` of the
+    head, ``load_checkpoint``, ``train`` with the same seed."""
     cls, lr, n_epochs, _, val_every, save_every, _ = TASKS[task]
     model = (cls() if model is None else model).to(device)
     freeze_backbone(model, train_backbone)
+    from . import heads
     if dropout_seed is not None:
-        from . import heads
         head = getattr(model.backbone, model.head_key)
         if not heads.counter_dropout(head, dropout_seed):
             raise ValueError("dropout_seed: the head (%s) has no Linear, Dropout in a Sequential" % model.head_key)
@@ -281,12 +282,20 @@ def train(task, train_loader, val_loader, device, save_dir, epochs=None, model=N
                 g["lr"] *= 0.5
                 log("Updated learning rate: {}".format(g["lr"]))
         if epoch % save_every == 0:
-            torch.save({"epoch": epoch, "model_state_dict": model.state_dict(), "optimizer_state_dict": optimizer.state_dict()},
-                       os.path.join(save_dir, "cnn_{}.pth".format(epoch)))
+            state = {"epoch": epoch, "model_state_dict": model.state_dict(), "optimizer_state_dict": optimizer.state_dict()}
+            if heads.dropout_state(model):
+                state["dropout_state"] = heads.dropout_state(model)
+            torch.save(state, os.path.join(save_dir, "cnn_{}.pth".format(epoch)))
     return model
 
 
 def load_checkpoint(model, path, device="cpu"):
-    """validate.py:37-38: ``torch.load(path)['model_state_dict']``"""
-    model.load_state_dict(torch.load(path, map_location=device)["model_state_dict"])
+    """validate.py:37-38: ``torch.load(path)['model_state_dict']``.  A model whose head draws its dropout under a seed (``heads.counter_dropout``) takes over
+    seed and step of a checkpoint that holds them: ``train`` with that seed goes on with the masks that follow."""
+    state = torch.load(path, map_location=device)
+    model.load_state_dict(state["model_state_dict"])
+    if "dropout_state" in state:
+        from . import heads
+        if heads.dropout_state(model):
+            heads.load_dropout_state(model, state["dropout_state"])
     return model

@@ -180,6 +180,28 @@ def counter_dropout(module, seed):
     return count
 
 
+def _counted(module):
+    return {name: m for name, m in module.named_modules() if isinstance(m, LinearDropout) or (isinstance(m, Mx4LinearLayer) and m.p)}
+
+
+def dropout_state(module):
+    """{qualified name: {"seed", "step"}} of the counter-based dropouts under ``module``, plain numbers: what a checkpoint keeps beside the state dict"""
+    return {name: {"seed": m.seed, "step": int(m.step)} for name, m in _counted(module).items()}
+
+
+def load_dropout_state(module, state):
+    """The counter-based dropouts under ``module`` go on from where those of ``state`` (``dropout_state``) stood; the two must name the same layers."""
+    layers = _counted(module)
+    if sorted(layers) != sorted(state):
+        raise ValueError("load_dropout_state: the module's dropouts (%s) are not the state's (%s)" % (", ".join(sorted(layers)), ", ".join(sorted(state))))
+    for name, m in layers.items():
+        m.seed = int(state[name]["seed"])
+        if isinstance(m.step, torch.Tensor):
+            m.step.fill_(state[name]["step"])
+        else:
+            m.step = int(state[name]["step"])
+
+
 def mx4_linears(module, prefix="", fuse_relu=True):
     """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (``fuse_relu``: a ReLU that follows it in an
     ``nn.Sequential``, a Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear`` stay (``float_linears``

@@ -357,3 +357,36 @@ def test_hip_float_weights_loaded_into_a_layer_that_has_run():
             layer.load_state_dict(nn.Linear(299, 70).state_dict())
         # (as any module's: of a state that does not fit, the tensors that do - the bias - are taken before the error)
         assert torch.equal(layer(x), ops.mx4_linear(x, ops.mx4_quantize(b.weight.detach()), layer.bias))
+
+
+# ---------------------------------------------------------------------------------------------------------------- going on from a checkpoint
+def test_training_goes_on_from_a_checkpoint_with_the_masks_that_follow(on_the_cpu, tmp_path):
+    from eval_driving_safety_amd import classifiers as C
+
+    def model():
+        return holder(nn.Sequential(small_head(8), nn.Linear(3, 1), nn.Dropout(0.1), nn.Sigmoid()))
+
+    def run(m, data, where):
+        return C.train("dynamic_vehicles", data, None, torch.device("cpu"), str(tmp_path / where), epochs=1, model=m, log=lambda *a: None, dropout_seed=9)
+
+    data = [(rows(4, k), torch.tensor([0.0, 1.0, 1.0, 0.0])) for k in range(5)]
+    m = run(model(), data[:3], "a")
+    saved = torch.load(tmp_path / "a" / "cnn_1.pth")
+    assert [v["step"] for v in saved["dropout_state"].values()] == [3, 3, 3] and list(saved["model_state_dict"]) == list(model().state_dict())
+    on = model()
+    heads.counter_dropout(on.net.fc, 9)
+    C.load_checkpoint(on, tmp_path / "a" / "cnn_1.pth")
+    for q in (m, on):
+        run(q, data[3:], "b")
+    assert heads.dropout_state(m) == heads.dropout_state(on) and all(v["step"] == 5 for v in heads.dropout_state(on).values())
+    assert all(torch.equal(a, b) for a, b in zip(m.state_dict().values(), on.state_dict().values()))
+    plain = C.load_checkpoint(model(), tmp_path / "a" / "cnn_1.pth")              # without counter-based layers: the weights alone
+    assert heads.dropout_state(plain) == {}
+    C.train("dynamic_vehicles", data[:1], None, torch.device("cpu"), str(tmp_path / "c"), epochs=1, model=plain, log=lambda *a: None)
+    assert "dropout_state" not in torch.load(tmp_path / "c" / "cnn_1.pth")
+    layer = on.net.fc[0][0]
+    layer.step = torch.zeros(1, dtype=torch.int64)
+    C.load_checkpoint(on, tmp_path / "a" / "cnn_1.pth")
+    assert int(layer.step) == 3
+    with pytest.raises(ValueError, match="not the state's"):
+        heads.load_dropout_state(on, {"fc": {"seed": 1, "step": 1}})
