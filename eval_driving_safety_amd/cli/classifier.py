@@ -27,7 +27,12 @@ def build_parser():
 
 
 def main(argv=None):
-    args = build_parser().parse_args(argv)
+    parser = build_parser()
+    args = parser.parse_args(argv)
+    if args.mode == "validate" and args.dropout_seed is not None:
+        parser.error("--dropout_seed is for train: nothing is dropped in validate")
+    if args.mode == "train" and args.head != "float32":
+        parser.error("--head %s is for validate: a head is trained in float32" % args.head)
     cls, _, _, batch, _, _, flip = C.TASKS[args.task]
     dev = torch.device(args.device if args.device else ("cuda" if torch.cuda.is_available() else "cpu"))      # train.py:11
     dyn = args.task == "dynamic_vehicles"

@@ -390,3 +390,11 @@ def test_training_goes_on_from_a_checkpoint_with_the_masks_that_follow(on_the_cp
     assert int(layer.step) == 3
     with pytest.raises(ValueError, match="not the state's"):
         heads.load_dropout_state(on, {"fc": {"seed": 1, "step": 1}})
+
+
+def test_the_command_refuses_options_of_the_other_mode(capsys):
+    from eval_driving_safety_amd.cli import classifier
+    for argv, word in ((["dynamic_vehicles", "validate", "--dropout_seed", "7"], "--dropout_seed"), (["driving_constraint", "train", "--head", "mxfp4"], "--head")):
+        with pytest.raises(SystemExit) as e:
+            classifier.main(argv)
+        assert e.value.code == 2 and word + " " in capsys.readouterr().err
