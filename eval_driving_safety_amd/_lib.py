@@ -182,6 +182,9 @@ def _open(path):
             "g.build()'` or `make -C eval_driving_safety_amd/csrc` (needs hipcc, targets gfx950). "
             "This package has no CPU / PyTorch fallback." % (os.path.basename(path), path))
     lib = ctypes.CDLL(path)
+    missing = [name for name in EXPORTED if not hasattr(lib, name)]
+    if missing:                          # (a build of other sources: entry points may have joined since without a new ABI version)
+        raise ImportError("%s lacks %s%s - rebuild" % (os.path.basename(path), missing[0], " and %d more entry points" % (len(missing) - 1) if missing[1:] else ""))
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
