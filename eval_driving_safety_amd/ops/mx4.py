@@ -138,15 +138,21 @@ def mx4_linear_dgrad(grad_y, w, mask=None):
     return gx
 
 
+def _stamp(w):
+    """moves on with every in-place change of the weight's tensors (those made in inference mode do not count theirs)"""
+    return tuple(None if t.is_inference() else t._version for t in (w.codes, w.scales))
+
+
 class Mx4Linear(torch.autograd.Function):
-    """``Mx4Linear.apply(x, w, bias=None, relu=False)``: ``mx4_linear`` with its gradient w.r.t. ``x``; weight and bias are constants of a frozen head"""
+    """``Mx4Linear.apply(x, w, bias=None, relu=False)``: ``mx4_linear`` with its gradient w.r.t. ``x``; weight and bias are constants of a frozen head
+    (a weight whose tensors were changed in place between the forward and the backward pass is refused, as autograd refuses it of its own)"""
 
     @staticmethod
     def forward(ctx, x, w, bias=None, relu=False):
         if ctx.needs_input_grad[2]:
             raise ValueError("Mx4Linear has no gradient w.r.t. its bias (a frozen head): detach it")
         y = mx4_linear(x, w, bias, relu)
-        ctx.w = w
+        ctx.w, ctx.stamp = w, _stamp(w)
         ctx.save_for_backward(y if relu else None)
         return y
 
@@ -154,6 +160,8 @@ class Mx4Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
         y, = ctx.saved_tensors
+        if _stamp(ctx.w) != ctx.stamp:
+            raise RuntimeError("Mx4Linear: the weight was changed in place after the forward pass: its gradient would be another layer's")
         return mx4_linear_dgrad(grad_y.contiguous(), ctx.w, y), None, None, None
 
 

@@ -398,3 +398,23 @@ def test_the_command_refuses_options_of_the_other_mode(capsys):
         with pytest.raises(SystemExit) as e:
             classifier.main(argv)
         assert e.value.code == 2 and word + " " in capsys.readouterr().err
+
+
+# ---------------------------------------------------------------------------------------------------------------- weights between the passes
+def test_a_weight_changed_between_the_passes_is_refused(monkeypatch):
+    from eval_driving_safety_amd import ops
+    from eval_driving_safety_amd.ops import mx4
+    monkeypatch.setattr(mx4, "mx4_linear", lambda x, w, bias, relu: x.detach()[:, :w.rows].clone())
+    monkeypatch.setattr(mx4, "mx4_linear_dgrad", lambda g, w, mask: torch.nn.functional.pad(g, (0, w.cols - w.rows)))
+    for inference in (False, True):
+        with torch.inference_mode(inference):
+            w = ops.Mx4(torch.zeros((1, 5, 128), dtype=torch.uint8), torch.zeros((1, 5, 8), dtype=torch.uint8), (5, 24))
+        x = rows(3).requires_grad_()
+        ops.Mx4Linear.apply(x, w).sum().backward()
+        assert bool((x.grad[:, :5] == 1).all()) and not x.grad[:, 5:].any()
+    for name in ("codes", "scales"):
+        w = ops.Mx4(torch.zeros((1, 5, 128), dtype=torch.uint8), torch.zeros((1, 5, 8), dtype=torch.uint8), (5, 24))
+        y = ops.Mx4Linear.apply(x, w)
+        getattr(w, name).add_(1)
+        with pytest.raises(RuntimeError, match="changed in place"):
+            y.sum().backward()
