@@ -82,7 +82,7 @@ class Dropout(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
         y, step = ctx.saved_tensors
-        gx, gbias = dropout_bwd(grad_y.contiguous(), ctx.p, ctx.seed, ctx.step if step is None else step, y, ctx.needs_input_grad[4])
+        gx, gbias = dropout_bwd(grad_y.contiguous(), ctx.p, ctx.seed, ctx.step if step is None else step, y, any(ctx.needs_input_grad[4:]))      # (what follows seed may be left out)
         return gx, None, None, None, gbias, None
 
 

@@ -149,7 +149,7 @@ class Mx4Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias=None, relu=False):
-        if ctx.needs_input_grad[2]:
+        if any(ctx.needs_input_grad[2:]):            # (bias and relu may be left out)
             raise ValueError("Mx4Linear has no gradient w.r.t. its bias (a frozen head): detach it")
         y = mx4_linear(x, w, bias, relu)
         ctx.w, ctx.stamp = w, _stamp(w)

@@ -418,3 +418,41 @@ def test_a_weight_changed_between_the_passes_is_refused(monkeypatch):
         getattr(w, name).add_(1)
         with pytest.raises(RuntimeError, match="changed in place"):
             y.sum().backward()
+
+
+# ---------------------------------------------------------------------------------------------------------------- arguments left out
+def test_autograd_functions_with_the_arguments_left_out_that_may_be(monkeypatch):
+    from eval_driving_safety_amd import ops
+    from eval_driving_safety_amd.ops import dropout, mx4
+    monkeypatch.setattr(dropout, "dropout", lambda x, p, seed, step, bias, relu: torch.tensor(O.dropout(x.detach().numpy(), p, seed, step)).float())
+    monkeypatch.setattr(dropout, "dropout_bwd", lambda g, p, seed, step, y, with_bias: (torch.tensor(O.dropout_bwd(g.numpy(), p, seed, step)[0]).float(), None))
+    for extra in ((), (3,), (3, None), (3, None, False)):
+        x = rows(4).requires_grad_()
+        ops.Dropout.apply(x, 0.5, 7, *extra).sum().backward()
+        kept = O.dropout_kept(0, 96, 0.5, 7, 3 if extra else 0).reshape(4, 24)
+        assert np.array_equal(x.grad.numpy(), kept * 2.0)
+    monkeypatch.setattr(mx4, "mx4_linear", lambda x, w, bias, relu: x.detach()[:, :w.rows].clone())
+    monkeypatch.setattr(mx4, "mx4_linear_dgrad", lambda g, w, mask: torch.nn.functional.pad(g, (0, w.cols - w.rows)))
+    w = ops.Mx4(torch.zeros((1, 5, 128), dtype=torch.uint8), torch.zeros((1, 5, 8), dtype=torch.uint8), (5, 24))
+    for extra in ((), (None,), (None, False), (torch.zeros(5),)):
+        x = rows(3).requires_grad_()
+        ops.Mx4Linear.apply(x, w, *extra).sum().backward()
+        assert bool((x.grad[:, :5] == 1).all()) and not x.grad[:, 5:].any()
+    with pytest.raises(ValueError):
+        ops.Mx4Linear.apply(rows(3), w, torch.zeros(5, requires_grad=True))
+
+
+@pytest.mark.gpu
+def test_hip_autograd_functions_with_the_arguments_left_out_that_may_be():
+    from eval_driving_safety_amd import ops
+    x = rows(4).cuda().requires_grad_()
+    g, = torch.autograd.grad(ops.Dropout.apply(x, 0.5, 7).sum(), x)
+    assert torch.equal(g, ops.dropout_bwd(torch.ones_like(x), 0.5, 7)[0])
+    w = ops.mx4_quantize(rows(5, 2).cuda())
+    g, = torch.autograd.grad(ops.Mx4Linear.apply(x, w).sum(), x)
+    assert torch.equal(g, ops.mx4_linear_dgrad(torch.ones((4, 5), device="cuda"), w))
+    w.codes.zero_()
+    y = ops.Mx4Linear.apply(x, w)
+    w.scales.add_(1)
+    with pytest.raises(RuntimeError, match="changed in place"):
+        y.sum().backward()
