@@ -423,7 +423,8 @@ def test_a_weight_changed_between_the_passes_is_refused(monkeypatch):
 # ---------------------------------------------------------------------------------------------------------------- arguments left out
 def test_autograd_functions_with_the_arguments_left_out_that_may_be(monkeypatch):
     from eval_driving_safety_amd import ops
-    from eval_driving_safety_amd.ops import dropout, mx4
+    import sys
+    dropout, mx4 = sys.modules["eval_driving_safety_amd.ops.dropout"], sys.modules["eval_driving_safety_amd.ops.mx4"]
     monkeypatch.setattr(dropout, "dropout", lambda x, p, seed, step, bias, relu: torch.tensor(O.dropout(x.detach().numpy(), p, seed, step)).float())
     monkeypatch.setattr(dropout, "dropout_bwd", lambda g, p, seed, step, y, with_bias: (torch.tensor(O.dropout_bwd(g.numpy(), p, seed, step)[0]).float(), None))
     for extra in ((), (3,), (3, None), (3, None, False)):
