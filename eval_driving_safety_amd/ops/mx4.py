@@ -3,6 +3,12 @@
 from ._lowp import *       # noqa: F401,F403  (torch, _lib and the argument helpers)
 
 _PANEL = 256               # columns of a panel of the layout: 128 code bytes and 8 scale bytes a row
+_MOST = 1 << 20            # rows, and columns, of a matrix that the kernels index
+
+
+def _fits(rows, cols, name):
+    if rows > _MOST or cols > _MOST:
+        raise ValueError("%s: an MXFP4 matrix has at most 2**20 rows (all leading dimensions together) and 2**20 columns, got %d x %d: take it in parts" % (name, rows, cols))
 
 
 class Mx4:
@@ -53,11 +59,13 @@ def _mx4(q, name):
 
 def mx4_quantize(x):
     """``x`` [..., C] float32 / bfloat16 / float16 -> Mx4 (adv_mx4_quantize): per 32 consecutive values of a row the power of two that puts the
-    largest magnitude into [4, 8), nearest 4-bit value (ties to even, beyond 6 saturated).  A block with a NaN or an infinity becomes NaN."""
+    largest magnitude into [4, 8), nearest 4-bit value (ties to even, beyond 6 saturated).  A block with a NaN or an infinity becomes NaN.  At most 2**20
+    rows and 2**20 columns."""
     _head(x, "x")
     rows, cols = _matrix(x)
     if cols < 1:
         raise ValueError("x needs at least one column")
+    _fits(rows, cols, "x")
     panels = (cols + _PANEL - 1) // _PANEL
     codes, scales = x.new_empty((panels, rows, 128), dtype=torch.uint8), x.new_empty((panels, rows, 8), dtype=torch.uint8)
     if rows:
@@ -101,10 +109,11 @@ def mx4_linear(x, w, bias=None, relu=False, dtype=None):
     if len(x.shape) < 1 or x.shape[-1] != w.cols:
         raise ValueError("x %s does not fit a weight of %d columns" % (tuple(x.shape), w.cols))
     _same_device(w, x, bias)
-    y = w.codes.new_empty(x.shape[:-1] + (w.rows,), dtype=dtype)
-    if bias is not None and tuple(_head(bias, "bias", y).shape) != (w.rows,):
-        raise ValueError("bias must be [%d], got %s" % (w.rows, tuple(bias.shape)))
     m, n, k = x.shape[:-1].numel(), w.rows, w.cols
+    _fits(m, k, "x")
+    y = w.codes.new_empty(x.shape[:-1] + (n,), dtype=dtype)
+    if bias is not None and tuple(_head(bias, "bias", y).shape) != (n,):
+        raise ValueError("bias must be [%d], got %s" % (n, tuple(bias.shape)))
     held = _mx4(x, "x") if isinstance(x, Mx4) else None
     if not (m and n):
         return y
@@ -116,9 +125,9 @@ def mx4_linear(x, w, bias=None, relu=False, dtype=None):
 
 
 def mx4_linear_dgrad(grad_y, w, mask=None):
-    """the gradient of ``mx4_linear`` w.r.t. ``x`` -> [..., K], straight through x's quantisation (adv_mx4_linear_dgrad): ``(grad_y where mask > 0) . W``
-    with ``mask`` the layer's output where it had a ReLU, else None.  ``grad_y`` [..., N] float32 / bfloat16 / float16 enters exactly (bits of a float32 under
-    2**-133 are cut); sums are float32."""
+    """the gradient of ``mx4_linear`` w.r.t. ``x`` -> [..., K], straight through x's quantisation (adv_mx4_linear_dgrad): ``(0 where mask <= 0, else
+    grad_y) . W`` with ``mask`` the layer's output where it had a ReLU, else None.  ``grad_y`` [..., N] float32 / bfloat16 / float16 enters exactly (bits of
+    a float32 under 2**-133 are cut); sums are float32."""
     _mx4(w, "w")
     _head(grad_y, "grad_y")
     if len(w.shape) != 2 or grad_y.dim() < 1 or grad_y.shape[-1] != w.rows:
@@ -126,8 +135,9 @@ def mx4_linear_dgrad(grad_y, w, mask=None):
     if mask is not None and _head(mask, "mask", grad_y).shape != grad_y.shape:
         raise ValueError("mask must have grad_y's shape")
     _same_device(w, grad_y)
-    gx = grad_y.new_empty(grad_y.shape[:-1] + (w.cols,))
-    m, n, k, kind = grad_y.shape[:-1].numel(), w.rows, w.cols, _FLOATS[gx.dtype]
+    m, n, k, kind = grad_y.shape[:-1].numel(), w.rows, w.cols, _FLOATS[grad_y.dtype]
+    _fits(m, k, "grad_y")
+    gx = grad_y.new_empty(grad_y.shape[:-1] + (k,))
     if not m:
         return gx
     if not n:
