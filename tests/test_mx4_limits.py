@@ -23,3 +23,13 @@ def test_hip_matrices_of_too_many_rows_are_refused_with_the_reason():
         with pytest.raises(ValueError, match="take it in parts"):
             call()
     assert ops.mx4_linear(tall[:-1], w).shape == (1 << 10, 1 << 10, 4)
+
+
+def test_oracle_at_the_end_of_the_scales_range():
+    """blocks whose scale is held at 2^-127: what lies on that scale's grid is kept, what lies under its first midpoint is gone"""
+    kept = np.ldexp(np.array([[6.0, 3.0, 1.5, 0.5, -2.0]]), -127).astype(np.float32)
+    assert np.array_equal(O.mx4_values(kept), kept.astype(np.float64))
+    for e in (-130, -140, -149):                       # the largest: 6 * 2^-130 = 0.75 * 2^-127, a tie that goes to 1 * 2^-127
+        x = np.ldexp(np.array([[6.0, 2.0, 1.5, 0.5, -4.0]]), e).astype(np.float32)
+        want = np.ldexp(np.array([[1.0, 0.0, 0.0, 0.0, -0.5]]), -127) if e == -130 else np.zeros((1, 5))
+        assert np.array_equal(O.mx4_values(x), want), e
