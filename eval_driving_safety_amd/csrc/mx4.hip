@@ -740,29 +740,43 @@ int64_t padded(int64_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
 //   thin   one launch, but every 16 rows of W read all of x again: up to 16 rows of up to 56 panels (8 rows of 8192 x 4096: 7.7 against 9.2 us, of
 //          12544 x 2048 9.3 against 9.5, of 25088 x 4096 17.0 against 13.9), a single row of up to 112, which is quantised in there (25088: 15.5 against
 //          17.5), and up to 64 rows of 1024 panels together under a small weight (32 of 6400 x 1024: 7.6 against 7.7, 64 of them 11.4 against 8.6).
-//   big    256 x 256 tiles where there are 128 of them or more, else 128 x 128, of which 64 or 32 rows where x has no more (32 x 25088 x 4096: 20.2 ->
-//          14.3 us with its join).
+//   big    256 x 256 tiles, whole or with their panels dealt to two workgroups, or 128 x 128, of which 64 or 32 rows where x has no more: what is estimated
+//          to take less.  A round of 256 workgroups takes, for each panel, 0.94 - 1.68 us (big; more once they crowd) or 0.27 - 0.55 (128 rows), and 11.5
+//          or 5.1 us for its start and end; a part 1.2 us per million sums to join.  x quantised before, bfloat16, 25088 -> 4096: 2048 rows big in two parts
+//          113 us, whole 132, 128 rows 117; 2049 to 4096 rows big 131 .. 178, 128 rows 156 .. 241, in two parts 166 .. 219; 4097 rows 128 rows 270,
+//          big 283; 1500 rows big in two parts 95, 128 rows 105.  4096 -> 4096: 2048 rows 128 rows 28, big 33, in two parts 43.  Up to 128 rows of x never
+//          fill half of a big tile: 20 of 25088 -> 32768 take 70 us in tiles of 32 rows, 153 (in two parts 109) in big ones, 128 of them 83 and 156.
 //   splits the panels are dealt to several workgroups a tile where tiles alone do not fill the chip: the number with the least estimated time, from
 //          what a panel takes (128 rows: 0.26 us up to 64 workgroups, 0.45 at one a CU; fewer rows 0.14 and 0.33), three panels' time for a workgroup's
-//          start and end, and the joining pass.  Fitted to 8 .. 512 rows of nine weights: within 1.3 % of the best count on average.
+//          start and end, and the joining pass.  Fitted to 8 .. 512 rows of nine weights.
 struct LinearPlan {
   int thin, big, splits;
 };
+// us for ``groups`` workgroups of ``panels`` panels each, a panel taking ``first`` us + ``more`` for every workgroup at work, + ``crowd`` for each beyond 144
+double estimate_rounds(int64_t groups, int64_t panels, double first, double more, double crowd, double ends) {
+  auto round = [&](int64_t at_work) {
+    return ends + static_cast<double>(panels) * (first + more * static_cast<double>(at_work) + crowd * static_cast<double>(at_work > 144 ? at_work - 144 : 0));
+  };
+  return static_cast<double>(groups / 256) * round(256) + (groups % 256 ? round(groups % 256) : 0.0);
+}
+double estimate_join(int64_t m, int64_t n, int64_t splits) { return splits > 1 ? 1.0 + 1.2e-6 * static_cast<double>(splits * m * n) : 0.0; }
 LinearPlan plan_linear(int64_t m, int64_t n, int64_t k) {
   const int64_t panels = panels_of(k);
   if (m * panels <= 112 || (m <= 16 ? panels <= 56 : m <= 64 && m * panels <= 1024 && n <= 4096)) return {1, 0, 1};
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
-  if (big >= 128) return {0, 1, static_cast<int>(big >= 256 || panels < 8 ? 1 : 256 / big)};
   int best = 1;
   double least = 0.0;
-  for (int64_t s = 1; s <= 32 && (s == 1 || s <= panels / 4); ++s) {
+  for (int64_t s = 1; s <= 32 && (s == 1 || (s <= panels / 4 && small <= 1024)); ++s) {
     const int64_t groups = small * s;
     const double panel = (m <= 64 ? 0.14 : 0.26) + 0.001 * static_cast<double>(groups <= 64 ? 0 : (groups < 256 ? groups - 64 : 192));
-    double t = panel * static_cast<double>(((panels + s - 1) / s + 3) * ((groups + 255) / 256));
-    if (s > 1) t += 1.0 + 1.2e-6 * static_cast<double>(s * m * n);
+    const double t = panel * static_cast<double>(((panels + s - 1) / s + 3) * ((groups + 255) / 256)) + estimate_join(m, n, s);
     if (s == 1 || t < least) best = static_cast<int>(s), least = t;
   }
-  return {0, 0, best};
+  if (m <= 128) return {0, 0, best};
+  const double with_small = estimate_rounds(small * best, (panels + best - 1) / best, 0.27, 0.00108, 0.0, 5.1) + estimate_join(m, n, best);
+  auto with_big = [&](int64_t s) { return estimate_rounds(big * s, (panels + s - 1) / s, 0.93, 0.002, 0.0021, 11.5) + estimate_join(m, n, s); };
+  const int parts = panels >= 8 && big <= 256 && with_big(2) < with_big(1) ? 2 : 1;
+  return with_small < 0.97 * with_big(parts) ? LinearPlan{0, 0, best} : LinearPlan{0, 1, parts};      // (the estimates are good to a few per cent)
 }
 int64_t linear_partial_bytes(int64_t m, int64_t n, int64_t k) {
   const LinearPlan p = plan_linear(m, n, k);
