@@ -485,7 +485,7 @@ __global__ __launch_bounds__(kBlock) void mx4_join(const float* __restrict__ par
       for (int j = 0; j < 4; ++j) v[j] += p[j];
     }
   }
-  int64_t c = !bias ? 0 : (n >> 32 ? i % cols : static_cast<int64_t>(static_cast<uint32_t>(i) % static_cast<uint32_t>(cols)));
+  int64_t c = bias ? static_cast<int64_t>(static_cast<uint32_t>(i) % static_cast<uint32_t>(cols)) : 0;      // (a result in parts has at most 2^24 elements: plan_linear, plan_dgrad)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (j >= left) break;
