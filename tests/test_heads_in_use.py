@@ -457,3 +457,46 @@ def test_hip_autograd_functions_with_the_arguments_left_out_that_may_be():
     w.scales.add_(1)
     with pytest.raises(RuntimeError, match="changed in place"):
         y.sum().backward()
+
+
+# ---------------------------------------------------------------------------------------------------------------- captured training
+@pytest.mark.gpu
+def test_hip_a_captured_forward_and_backward_draw_as_the_step_moves_on():
+    """a step of the layer and its gradients in one graph, replayed with the program's eager work between; then under activation recomputation, captured too"""
+    h = small_head(9).cuda()
+    heads.counter_dropout(h, 11)
+    layer = h[0].train()
+    layer.step = torch.zeros((1,), dtype=torch.int64, device="cuda")
+    x = rows(33, 5).cuda().requires_grad_()
+    g = torch.randn(33, 40, generator=torch.Generator().manual_seed(5)).cuda()
+
+    def step(recompute):
+        y = checkpoint(layer, x, use_reentrant=False, preserve_rng_state=False) if recompute else layer(x)
+        return (y.detach(),) + torch.autograd.grad(y, (x, layer.weight, layer.bias), g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for recompute in (False, True):
+            step(recompute)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for recompute in (False, True):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(recompute)
+        graphs.append((graph, out))
+    seen = []
+    for k in (4, 9, 4, 6):
+        layer.step.fill_(k)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = step(False)
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, eager)), k
+        kept = O.dropout_kept(0, 33 * 40, 0.5, layer.seed, k).reshape(33, 40)
+        assert not eager[0].cpu().numpy()[~kept].any()
+        seen.append(eager[1].clone())
+    assert torch.equal(seen[0], seen[2]) and not torch.equal(seen[0], seen[1])
