@@ -13,8 +13,9 @@ The attacks differentiate w.r.t. the images only; the detector is in eval mode a
   * a stride-2 1x1 layer (ResNet's down-sampling projections) is a sub-sampling copy + the 1x1 GEMM kernel;
   * layers without a kernel here (7x7 stems, strided 3x3 layers, grouped convolutions ...) keep torch's operator but still lose their
     BatchNorm (folded) and get bias + ReLU as ONE fused pass (``ops.bias_act_``);
-  * on request (``linear="mxfp4"``) every ``nn.Linear`` is evaluated and attacked as deployed in four bits: weights held in MXFP4, inputs quantised on
-    the way in, the gradient straight through (``heads.Mx4LinearLayer`` on csrc/mx4.hip);
+  * on request (``linear="mxfp4"``) every ``nn.Linear``, and every ``nn.Conv2d`` where its kernel covers the whole map it is given (the fully connected
+    layers of a RoI head), is evaluated and attacked as deployed in four bits: weights held in MXFP4, inputs quantised on the way in, the gradient
+    straight through (``heads.Mx4LinearLayer``, ``heads.Covering`` on csrc/mx4.hip);
   * gradients flow to the INPUT only: the adopted modules return no weight gradients (``adopt`` switches ``requires_grad`` off on
     what it adopts, as adapters._freeze does for the whole model).
 
@@ -35,6 +36,8 @@ import re
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from . import heads
 
 
 def fold_bn(weight, bias, bn, transposed=False):
@@ -155,6 +158,7 @@ class AdoptedConv2d(_Adopted):
         self.stride, self.dilation, self.groups = _pair(conv.stride), _pair(conv.dilation), conv.groups
         self.padding = _numeric_padding(conv)
         self.padding_mode = conv.padding_mode
+        self.covering = None                            # heads.Covering: this layer in four bits, wherever its kernel covers the map
         k = tuple(weight.shape[2:])
         s, p, d = _same(self.stride), (None if isinstance(self.padding, str) else _same(self.padding)), _same(self.dilation)
         self.subsample = self.groups == 1 and self.padding_mode == "zeros" and s == 2 and k == (1, 1) and p == 0 and d == 1      # strided 1x1: sub-sample + GEMM
@@ -165,6 +169,8 @@ class AdoptedConv2d(_Adopted):
     def forward(self, x):
         ops = self._ops(x)
         stride = self.stride
+        if self.covering is not None and not isinstance(self.padding, str) and heads.covers(x, self.weight, self.padding, self.dilation, self.groups):
+            return self.covering(x, self.weight, self.bias, self.relu)[:, :, None, None]
         if self.subsample and x.dtype == torch.float32:
             x = x[:, :, ::2, ::2].contiguous()          # every other pixel of every other row: what a stride-2 1x1 layer reads
             stride = (1, 1)                             # (also for torch's operator below, should the kernel refuse the sub-sampled map)
@@ -252,7 +258,8 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
     docstring).  ``functional``: also bind the two functional patterns of a DSGN forward - 5-D ``F.grid_sample`` and the
     ``F.interpolate(trilinear)`` -> softmax -> depth-weighted sum chain - to ``ops.GridSample3d`` / ``ops.DepthRegress`` by putting a proxy
     where the defining Python modules hold ``torch.nn.functional`` (adopt_functional.py; ``adopt_functional.unbind()`` undoes it).
-    ``linear="mxfp4"``: the model's ``nn.Linear`` layers with four-bit weights - another model, a few per cent off: give ``verify`` a ``tol`` to match.
+    ``linear="mxfp4"``: the model's ``nn.Linear`` layers, and its 2D convolutions where they cover their map, with four-bit weights - another model, a few
+    per cent off: give ``verify`` a ``tol`` to match.
     -> {"replaced": [(qualified name, what)], "folded_bn": n, "fused_relu": n, "kept": [(name, why)], "upsample_add": modules whose
     ``_upsample_add`` now has a deterministic backward, "functional": [(python module, global name)] rebound}."""
     if model.training:
@@ -262,7 +269,6 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
     if linear is not None and isinstance(model, nn.Linear):
         raise ValueError("adopt() replaces layers in the module that holds them: a %s by itself cannot be adopted" % type(model).__name__)
     if linear is not None:
-        from . import heads
         heads.refuse_hooked_linears(model)            # (before anything is replaced)
     before = rng = None
     if verify is not None:
@@ -315,6 +321,10 @@ def adopt(model, fuse_relu=True, fold_named_pairs=True, verify=None, tol=1e-4, f
             report["replaced"].append((_q(parent_name, name), getattr(parent, name).kind))
     if linear is not None:
         report["replaced"] += heads.mx4_linears(model, fuse_relu=fuse_relu)
+        from .surrogates import FoldedConv
+        for m in model.modules():
+            if isinstance(m, (AdoptedConv2d, FoldedConv)):
+                m.covering = heads.Covering()
     for name, m in model.named_modules():
         if isinstance(m, (nn.Conv1d, nn.Conv2d, nn.Conv3d, nn.ConvTranspose2d, nn.ConvTranspose3d)):
             report["kept"].append((name, type(m).__name__ + ": no libadvengine counterpart for this module type here"))

@@ -5,6 +5,7 @@ the product is torch's, bias + dropout + ReLU are one kernel (``ops.Dropout``), 
 ``Mx4LinearLayer`` stands for a frozen Linear (- ReLU) whose weight is held in MXFP4 (``ops.Mx4Linear``): gradients flow to its input only, as
 through every adopted layer."""
 import threading
+import types
 
 import torch
 import torch.nn as nn
@@ -127,6 +128,33 @@ class Mx4LinearLayer(_Counted, nn.Module):
 
     def extra_repr(self):
         return "%d -> %d, mxfp4%s%s" % (self.in_features, self.out_features, ", relu" if self.relu else "", ", p=%g, seed=%d" % (self.p, self.seed) if self.p else "")
+
+
+class Covering:
+    """A convolution whose kernel covers its whole map is a fully connected layer over the map's values (a detector's RoI head: 7x7 on the pooled grid, 1x1
+    behind it); whether it does shows when it runs.  Holds such a layer's weight in four bits, beside the float one of the module that asks."""
+
+    def __init__(self):
+        self.layer = self.weight = self.stamp = None
+
+    def __call__(self, x, weight, bias, relu):
+        """``relu?(x . weight + bias)`` [B, N] of ``x`` [B, C, kh, kw] under ``weight`` [N, C, kh, kw], which is quantised again where it was changed"""
+        from . import ops
+        stamp = None if weight.is_inference() else weight._version
+        if self.weight is not weight or self.stamp != stamp:
+            flat = weight.detach().flatten(1)
+            if self.layer is not None and self.layer.codes is not None and self.layer.codes.device == weight.device:
+                self.layer.load_state_dict({"weight": flat})             # (into the tensors that are there: a captured graph reads those)
+            else:
+                self.layer = Mx4LinearLayer(types.SimpleNamespace(in_features=flat.shape[1], out_features=flat.shape[0], weight=flat, bias=None))
+            self.weight, self.stamp = weight, stamp
+        bias = bias if bias is None or bias.dtype == x.dtype else bias.to(x.dtype)
+        return ops.Mx4Linear.apply(x.flatten(1), self.layer.held(), bias, bool(relu))
+
+
+def covers(x, weight, padding, dilation, groups):
+    """does the kernel of ``weight`` cover the whole map of ``x``, every value once?"""
+    return groups == 1 and x.shape[2:] == weight.shape[2:] and not any(padding) and (weight[0, 0].numel() == 1 or all(d == 1 for d in dilation))
 
 
 def _is_relu(m):

@@ -480,6 +480,7 @@ class FoldedConv(nn.Module):
         self.stride, self.padding, self.k = stride, padding, k
         self.flops = 0
         self._prep = None
+        self.covering = None      # heads.Covering (adopt(linear="mxfp4")): the layer in four bits, wherever its kernel covers the map
 
     def chainable(self):
         """on the ops.Conv2dAuto path (whose backward can take over the ReLU mask of its producer / leave its own to its consumer)?"""
@@ -499,7 +500,10 @@ class FoldedConv(nn.Module):
         if ho == 1 and wo == 1 and self.padding == 0 and self.k == x.shape[2] == x.shape[3]:
             # the kernel covers the whole map (the RoI head's 7x7 "fully connected" convolution, and the 1x1 behind it): one GEMM over
             # the rois.  (MIOpen's backward-data for [512,512,7,7] x [2048,512,7,7] takes 24 ms - 2 TFLOP/s; the GEMM 0.6 ms.)
-            y = F.linear(x.flatten(1), self.weight.flatten(1), self.bias)
+            if self.covering is not None:
+                y = self.covering(x, self.weight, self.bias, bool(relu) and residual is None)
+            else:
+                y = F.linear(x.flatten(1), self.weight.flatten(1), self.bias)
             if residual is not None:
                 y = y + residual.flatten(1)
             return (F.relu(y) if relu else y)[:, :, None, None]

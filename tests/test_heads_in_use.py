@@ -500,3 +500,71 @@ def test_hip_a_captured_forward_and_backward_draw_as_the_step_moves_on():
         assert not eager[0].cpu().numpy()[~kept].any()
         seen.append(eager[1].clone())
     assert torch.equal(seen[0], seen[2]) and not torch.equal(seen[0], seen[1])
+
+
+# ---------------------------------------------------------------------------------------------------------------- convolutions that are fully connected
+def test_which_convolutions_cover_their_map():
+    x = torch.zeros(2, 3, 7, 5)
+    yes = lambda w, p=(0, 0), d=(1, 1), g=1, m=x: heads.covers(m, torch.zeros(w), p, d, g)      # noqa: E731
+    assert yes((4, 3, 7, 5)) and yes((4, 3, 1, 1), d=(2, 2), m=torch.zeros(2, 3, 1, 1))
+    assert not yes((4, 3, 7, 7)) and not yes((4, 3, 7, 5), p=(1, 1)) and not yes((4, 3, 7, 5), d=(2, 2)) and not yes((3, 1, 7, 5), g=3)
+    assert not yes((4, 3, 1, 1))
+
+
+@pytest.mark.gpu
+def test_hip_an_adopted_roi_heads_fully_connected_convolutions_are_in_four_bits():
+    """7x7 convolution on the pooled grid - ReLU - 1x1 - ReLU, as a Stereo R-CNN head has them: each layer the four-bit product of its own input, the
+    gradient straight through; on another map the same layer keeps its float convolution"""
+    from eval_driving_safety_amd import adopt as A, ops
+    torch.manual_seed(10)
+    net = nn.Sequential(nn.Conv2d(8, 48, 7, stride=7), nn.ReLU(), nn.Conv2d(48, 40, 1), nn.ReLU()).eval().cuda()
+    w = [net[0].weight.detach().flatten(1).clone(), net[2].weight.detach().flatten(1).clone()]
+    b = [net[0].bias.detach().clone(), net[2].bias.detach().clone()]
+    plain = [p.detach().clone() for p in (net[0].weight, net[0].bias)]
+    A.adopt(net, linear="mxfp4", functional=False)
+    assert [(n, m.relu) for n, m in net.named_children() if isinstance(m, A.AdoptedConv2d)] == [("0", True), ("2", True)]
+    x = torch.randn(33, 8, 7, 7, generator=torch.Generator().manual_seed(10)).cuda().requires_grad_()
+    y = net(x)
+    q = [ops.mx4_quantize(v) for v in w]
+    z1 = ops.mx4_linear(x.detach().flatten(1), q[0], b[0], True)
+    z2 = ops.mx4_linear(z1, q[1], b[1], True)
+    assert y.shape == (33, 40, 1, 1) and torch.equal(y.flatten(1), z2)
+    g = torch.randn(33, 40, generator=torch.Generator().manual_seed(11)).cuda()
+    y.backward(g[:, :, None, None])
+    gx = ops.mx4_linear_dgrad(ops.mx4_linear_dgrad(g, q[1], z2), q[0], z1)
+    assert torch.equal(x.grad.flatten(1), gx) and gx.abs().max() > 0
+    far = torch.randn(2, 8, 14, 7, generator=torch.Generator().manual_seed(12)).cuda()
+    with torch.no_grad():
+        want = torch.relu(nn.functional.conv2d(far.double(), plain[0].double(), plain[1].double(), stride=7))
+        # 392 float32 products and additions a value
+        assert bool(((net[0](far).double() - want).abs() <= 400 * 2.0 ** -23 * nn.functional.conv2d(far.double().abs(), plain[0].double().abs(), plain[1].double().abs(), stride=7)).all())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = net(x)
+        net[0].weight.mul_(2)                                                 # quantised again, into what the captured graph reads
+        z1 = ops.mx4_linear(x.detach().flatten(1), ops.mx4_quantize(2 * w[0]), b[0], True)
+        want = ops.mx4_linear(z1, q[1], b[1], True)
+        for _ in range(3):
+            assert torch.equal(net(x).flatten(1), want)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out.flatten(1), want)
+
+
+@pytest.mark.gpu
+def test_hip_the_surrogate_detectors_roi_head_in_four_bits():
+    from eval_driving_safety_amd import adopt as A, ops
+    from eval_driving_safety_amd.surrogates import StereoRcnnR101
+    net = StereoRcnnR101(blocks=(1, 1, 1, 1), rois_per_image=16).eval().cuda()
+    pooled = torch.relu(torch.randn(37, 512, 7, 7, generator=torch.Generator().manual_seed(13))).cuda().requires_grad_()
+    float_top = net.head_to_tail(pooled).detach()
+    A.adopt(net, linear="mxfp4", functional=False)
+    top = net.head_to_tail(pooled)
+    q7, q1 = [ops.mx4_quantize(m.weight.flatten(1).contiguous()) for m in (net.top7, net.top1)]
+    z7 = ops.mx4_linear(pooled.detach().flatten(1), q7, net.top7.bias, True)
+    z1 = ops.mx4_linear(z7, q1, net.top1.bias, True)
+    assert torch.equal(top, z1) and not torch.equal(top, float_top)
+    g = torch.randn(37, 2048, generator=torch.Generator().manual_seed(14)).cuda()
+    got, = torch.autograd.grad(top, pooled, g)
+    assert torch.equal(got.flatten(1), ops.mx4_linear_dgrad(ops.mx4_linear_dgrad(g, q1, z1), q7, z7))
+    assert isinstance(net.cls_score, heads.Mx4LinearLayer)
