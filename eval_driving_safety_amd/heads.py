@@ -149,7 +149,7 @@ class Covering:
                 self.layer = Mx4LinearLayer(types.SimpleNamespace(in_features=flat.shape[1], out_features=flat.shape[0], weight=flat, bias=None))
             self.weight, self.stamp = weight, stamp
         bias = bias if bias is None or bias.dtype == x.dtype else bias.to(x.dtype)
-        return ops.Mx4Linear.apply(x.flatten(1), self.layer.held(), bias, bool(relu))
+        return ops.Mx4Linear.apply(x.flatten(1).contiguous(), self.layer.held(), bias, bool(relu))
 
 
 def covers(x, weight, padding, dilation, groups):

@@ -568,3 +568,19 @@ def test_hip_the_surrogate_detectors_roi_head_in_four_bits():
     got, = torch.autograd.grad(top, pooled, g)
     assert torch.equal(got.flatten(1), ops.mx4_linear_dgrad(ops.mx4_linear_dgrad(g, q1, z1), q7, z7))
     assert isinstance(net.cls_score, heads.Mx4LinearLayer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("boxes", [0, 1, 5])
+def test_hip_covering_layers_on_slices_of_maps_and_without_boxes(boxes):
+    from eval_driving_safety_amd import adopt as A
+    torch.manual_seed(15)
+    net = nn.Sequential(nn.Conv2d(8, 6, 1), nn.ReLU()).eval().cuda()
+    A.adopt(net, linear="mxfp4", functional=False)
+    whole = torch.randn(boxes, 16, 1, 1, generator=torch.Generator().manual_seed(15)).cuda()
+    for x in (whole[:, :8], whole[:, ::2], whole[:, 8:].contiguous(memory_format=torch.channels_last)):
+        xr = x.detach().requires_grad_()
+        y = net(xr)
+        assert y.shape == (boxes, 6, 1, 1) and torch.equal(y, net(x.clone().contiguous()))
+        y.sum().backward()
+        assert xr.grad.shape == x.shape
