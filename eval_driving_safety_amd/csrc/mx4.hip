@@ -309,8 +309,9 @@ __device__ __forceinline__ Float16 mfma(Uint4 a, Uint4 b, Float16 c, uint32_t sa
 // Many rows: BM x BN of y a workgroup of four waves (2 x 2, or side by side over 32 rows), 32x32x64 instructions; panels go to LDS by direct copies,
 // two (256 x 256) or three buffers, one barrier a panel.  A panel is four steps of 64 columns; the operands of a step are read while the step before is
 // multiplied, and the barrier stands before a panel's last step, whose operands are in registers by then - its products cover the first reads of the next
-// panel.  4096 x 25088 x 4096 in 166 us: 5.1 PFLOP/s of the 7.3 that the bare instruction reaches, the matrix pipe 0.76 busy.  The smaller tiles are
-// bound by how long a panel takes to come: with the third buffer 128 x 4096 x 4104 takes 15.1 us for 17.9, 32 x 25088 x 4096 17.5 for 19.7.
+// panel.  4096 x 25088 x 4096: 178 us in a kernel trace (median of 12, least 175): 4.7 PFLOP/s of the 7.0 - 7.6 that the bare instruction reaches, the matrix
+// pipe 0.76 busy; among other calls 166, the call's time less the quantisation's.  The smaller tiles are bound by how long a panel takes to come: with the
+// third buffer 128 x 4096 x 4104 takes 15.1 us for 17.9, 32 x 25088 x 4096 17.5 for 19.7 (calls).
 template <int BM, int BN>
 constexpr int kTileStages = BM > 128 ? 2 : 3;
 template <int BM, int BN>
@@ -552,7 +553,8 @@ __global__ __launch_bounds__(kBlock) void mx4_grad_terms(const T* __restrict__ g
 
 // LDS places of a stage.  Terms: rows of 64 bytes (32 of the contraction); four of them fill the banks, so chunk c of row r lies at c ^ (r / 4 % 4).
 // W: rows (n) of 512 bytes (a panel's 256 columns), in units of 16 bytes; what is written together - two rows, eight blocks of columns, the same unit
-// of each - and what a transposing read takes together - four rows, four neighbouring units - must lie in different banks.
+// of each - and what a transposing read takes together - four rows, four neighbouring units - must lie in different banks.  (By sixteen lanes they do;
+// the counters still show a third of the LDS cycles of 64-row tiles in bank conflicts, which this does not explain.)
 __device__ __forceinline__ int short_row(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
 __device__ __forceinline__ int wide_row(int row, int unit) { return row * 512 + ((unit ^ (row & 3) << 2 ^ (unit >> 4 & 1) ^ (row & 1) << 1) << 4); }
 
@@ -568,8 +570,9 @@ constexpr int kGradLds = 2 * (kPanel + N * BM) * 64;
 // Everything is doubled: while chunk c is multiplied, chunk c + 1 of W is taken from registers to LDS, the copies of its terms land, and the next kHeld
 // chunks of W are on their way to registers (one 16-byte and one byte load a thread and chunk: what a load instruction costs hardly depends on its
 // width).  One barrier a chunk.  The matrix instruction wants eight n of one column in a lane; the codes come along the columns: they are stored as
-// bfloat16 rows and turned by the transposing LDS read.  512 x 2048 to 25088 columns: 118 us in float32 (three terms: 1.34 PFLOP/s; the matrix pipe of a
-// busy CU 0.78 busy, 392 workgroups on 512 places).  37 x 4096 bfloat16: 22 us, bound by W's conversion.
+// bfloat16 rows and turned by the transposing LDS read.  512 x 2048 to 25088 columns: 132 us in float32 in a kernel trace (median of 12, least 129; three
+// terms: 1.2 PFLOP/s; the matrix pipe of a busy CU 0.78 busy, 392 workgroups on 512 places); among other calls 118, the call's time less the terms'.
+// 37 x 4096 bfloat16: 22 us, bound by W's conversion.
 constexpr int kHeld = 4;
 template <class T, int BM>
 __global__ __launch_bounds__(kBlock, BM == 128 ? 2 : 3) void mx4_dgrad(const uint8_t* __restrict__ planes, Operand w, T* __restrict__ gx, float* __restrict__ partial,
@@ -842,7 +845,8 @@ int run_linear(Operand x, const void* values, Operand w, const void* bias, void*
   return run_tile<T, 128, 128>(x, w, bias, y, partial, panels, p.splits, relu, st);
 }
 
-// The input gradient: the contraction is dealt to several workgroups where panels x row tiles do not fill two workgroups a CU
+// The input gradient: the contraction is dealt to several workgroups where panels x row tiles do not fill two workgroups a CU.  (Row tiles go by m alone,
+// and a part's joining has no price here: 301 rows of 4096 -> 25088, 294 workgroups, take 232 us where 512 take 250; 128 rows, in five parts, 81.)
 struct GradPlan {
   int bm, splits;
   int64_t padded_n;

@@ -39,7 +39,8 @@ class LinearDropout(_Counted, nn.Linear):
     number: set it to go on where another run stopped); in eval there is no dropout.  Training needs a ROCm device.  For a step captured in a
     hipGraph set ``step`` to an int64 CUDA tensor of one element and move it on between the replays (a number would repeat one mask: refused).  The same
     where activations are recomputed in the backward pass (torch.utils.checkpoint): the second forward must draw the first one's mask, so ``step`` has to
-    be a tensor that is moved on after the backward pass (a number has moved on by then: refused)."""
+    be a tensor that is moved on after the backward pass (a number has moved on by then: refused).  As with any module: no eager graph of its parameters
+    may be alive while a backward pass through it is captured."""
 
     def __init__(self, linear, p, seed, relu=False):
         nn.Module.__init__(self)
