@@ -141,7 +141,8 @@ class Covering:
     def __call__(self, x, weight, bias, relu):
         """``relu?(x . weight + bias)`` [B, N] of ``x`` [B, C, kh, kw] under ``weight`` [N, C, kh, kw], which is quantised again where it was changed"""
         from . import ops
-        stamp = None if weight.is_inference() else weight._version
+        # (in-place writes count the version up, ``weight.data = other`` - what ``module.to`` does - moves the pointer)
+        stamp = (weight.data_ptr(), weight.device, weight.dtype, None if weight.is_inference() else weight._version)
         if self.weight is not weight or self.stamp != stamp:
             flat = weight.detach().flatten(1)
             if self.layer is not None and self.layer.codes is not None and self.layer.codes.device == weight.device:
@@ -233,8 +234,8 @@ def load_dropout_state(module, state):
 
 def mx4_linears(module, prefix="", fuse_relu=True):
     """Replace, IN PLACE, every ``nn.Linear`` and ``LinearDropout`` under ``module`` by ``Mx4LinearLayer`` (``fuse_relu``: a ReLU that follows it in an
-    ``nn.Sequential``, a Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear`` stay (``float_linears``
-    names them).  -> [(qualified name, what)]"""
+    ``nn.Sequential``, a Dropout between them allowed, runs in its kernel: a dropped or scaled value keeps its sign).  Other subclasses of ``nn.Linear``
+    stay (``float_linears`` names them).  -> [(qualified name, what)]"""
     if type(module) in (nn.Linear, LinearDropout):
         raise ValueError("mx4_linears: a layer cannot be replaced in place without the module that holds it: build a heads.Mx4LinearLayer of it")
     refuse_hooked_linears(module, prefix)

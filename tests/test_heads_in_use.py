@@ -584,3 +584,32 @@ def test_hip_covering_layers_on_slices_of_maps_and_without_boxes(boxes):
         assert y.shape == (boxes, 6, 1, 1) and torch.equal(y, net(x.clone().contiguous()))
         y.sum().backward()
         assert xr.grad.shape == x.shape
+
+
+@pytest.mark.gpu
+def test_hip_a_covering_layer_follows_its_weight():
+    """written in place, given other memory, moved away and back, and to another type"""
+    from eval_driving_safety_amd import ops
+    gen = torch.Generator().manual_seed(16)
+    x = torch.randn(9, 8, 3, 3, generator=gen).cuda()
+    m = nn.Conv2d(8, 6, 3).cuda().requires_grad_(False)
+    covering = heads.Covering()
+
+    def check(x=x):
+        want = ops.mx4_linear(x.flatten(1), ops.mx4_quantize(m.weight.flatten(1)), m.bias, True)
+        assert torch.equal(covering(x, m.weight, m.bias, True), want)
+        return want
+
+    first = check()
+    m.weight.mul_(-1)
+    assert not torch.equal(check(), first)
+    m.weight.data = torch.randn(6, 8, 3, 3, generator=gen).cuda()
+    second = check()
+    m.cpu()
+    m.weight.mul_(2)
+    m.cuda()
+    assert not torch.equal(check(), second)
+    m.weight = nn.Parameter(torch.randn(6, 8, 3, 3, generator=gen).cuda(), requires_grad=False)
+    check()
+    m.half()
+    check(x.half())
